@@ -58,7 +58,10 @@ def build_hfk_hip():
             "-shared", "-fvisibility=hidden", "-Wall",
             # hipcc -O3 turns float code into packed-fp32 instructions on its own; keep them off.
             "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
-            "-I" + INCLUDE, "-I" + CSRC, os.path.join(CSRC, "hfk_capi.hip"), "-o", HFK_HIP_SO,
+            # half of the cores: the kernels' many types and shapes compile side by side
+            "-parallel-jobs=4",
+            "-I" + INCLUDE, "-I" + CSRC, os.path.join(CSRC, "hfk_capi.hip"), os.path.join(CSRC, "hfk_cache_ops.hip"),
+            os.path.join(CSRC, "hfk_attention.hip"), "-o", HFK_HIP_SO,
         ],
         quiet_patterns=("packed-fp32-ops' is not a recognized feature",),
     )
@@ -127,7 +130,8 @@ def build_pcie_through():
     os.makedirs(PCIE_LIB, exist_ok=True)
     _run(
         ["g++"] + cxx + incs
-        + ["-I" + INCLUDE, "-I" + CSRC, os.path.join(CSRC, "pcie_through_ops.cpp"), "-o", PCIE_THROUGH_SO]
+        + ["-I" + INCLUDE, "-I" + CSRC, os.path.join(CSRC, "pcie_through_ops.cpp"),
+           os.path.join(CSRC, "cache_ops_torch.cpp"), "-o", PCIE_THROUGH_SO]
         + link + ["-L" + PCIE_LIB, "-lhfk_hip", "-L" + COMMON, "-lmanaged_memory",
                   "-Wl,-rpath,$ORIGIN", "-Wl,-rpath,$ORIGIN/../../heterofusedkernels", "-Wl,-z,defs"]
     )

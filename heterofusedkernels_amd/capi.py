@@ -41,6 +41,12 @@ STATIC_STAGING_BYTES = 64 << 20
 ERR_STAGING_TOO_SMALL = -7
 ERR_TABLE_MISMATCH = -8
 ERR_STAGING_BUSY = -9
+ERR_BAD_TYPE = -10
+ERR_BAD_ALIGNMENT = -11
+ERR_WORKSPACE_TOO_SMALL = -12
+BF16 = 0
+FP16 = 1
+FP8_E4M3 = 2
 
 
 class KnobValue(ctypes.Structure):
@@ -55,6 +61,28 @@ class BlockMove(ctypes.Structure):
                 ("src_block_stride", ctypes.c_uint64), ("dst_block_stride", ctypes.c_uint64),
                 ("src_blocks", ctypes.c_uint64), ("dst_blocks", ctypes.c_uint64)]
 
+
+class CachePlane(ctypes.Structure):
+    """struct hfk_cache_plane."""
+    _fields_ = ([("values", ctypes.c_void_p), ("scales", ctypes.c_void_p)]
+                + [(n, ctypes.c_int64) for n in ("block_stride", "token_stride", "head_stride", "scale_block_stride",
+                                                 "scale_token_stride", "scale_head_stride")]
+                + [("blocks", ctypes.c_uint64)]
+                + [(n, ctypes.c_uint32) for n in ("block_tokens", "heads", "head_dim", "type")])
+
+
+class TokenRows(ctypes.Structure):
+    """struct hfk_token_rows."""
+    _fields_ = [("data", ctypes.c_void_p), ("token_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64),
+                ("type", ctypes.c_uint32)]
+
+
+class Attention(ctypes.Structure):
+    """struct hfk_attention."""
+    _fields_ = [("k", CachePlane), ("v", CachePlane), ("q", TokenRows), ("out", TokenRows), ("lse", ctypes.c_void_p),
+                ("n_rows", ctypes.c_uint64), ("q_heads", ctypes.c_uint32), ("scale", ctypes.c_float)]
+
+
 ENTRY_POINTS = (
     "hfk_version",
     "hfk_status_string",
@@ -68,6 +96,12 @@ ENTRY_POINTS = (
     "hfk_swap_blocks_staged_static",
     "hfk_swap_blocks_auto",
     "hfk_gather_blocks",
+    "hfk_cache_write",
+    "hfk_cache_read",
+    "hfk_prompt_attention",
+    "hfk_prompt_attention_workspace",
+    "hfk_prefix_attention",
+    "hfk_prefix_attention_workspace",
     "hfk_set_tuning",
     "hfk_get_tuning",
     "hfk_pace_state",
@@ -130,6 +164,17 @@ def load():
     L.hfk_swap_blocks_auto.restype = ci
     L.hfk_gather_blocks.argtypes = [vp, vp, vp, u32, u64, u64, u64, u64, u32, u32, vp]
     L.hfk_gather_blocks.restype = ci
+    plane, rows, attention = ctypes.POINTER(CachePlane), ctypes.POINTER(TokenRows), ctypes.POINTER(Attention)
+    for name in ("hfk_cache_write", "hfk_cache_read"):
+        getattr(L, name).argtypes = [plane, rows, plane, rows, vp, u64, vp]
+        getattr(L, name).restype = ci
+    for name in ("hfk_prompt_attention_workspace", "hfk_prefix_attention_workspace"):
+        getattr(L, name).argtypes = [attention, u64, u64, ctypes.POINTER(u64)]
+        getattr(L, name).restype = ci
+    L.hfk_prompt_attention.argtypes = [attention, vp, u64, u64, vp, vp, ci, vp, u64, vp]
+    L.hfk_prompt_attention.restype = ci
+    L.hfk_prefix_attention.argtypes = [attention, vp, u64, vp, vp, u64, vp, vp, u64, vp]
+    L.hfk_prefix_attention.restype = ci
     L.hfk_set_tuning.argtypes = [ci, i64]
     L.hfk_set_tuning.restype = ci
     L.hfk_get_tuning.argtypes = [ci]
@@ -219,6 +264,43 @@ def gather_blocks(dst_planes, src_planes, ids, n_planes, n_ids, block_bytes, src
                   workgroups=0, stream=0, flags=0):
     return load().hfk_gather_blocks(dst_planes, src_planes, ids, n_planes, n_ids, block_bytes, src_stride,
                                     src_blocks, flags, workgroups, stream)
+
+
+def _ref(struct):
+    return ctypes.byref(struct) if struct is not None else None
+
+
+def cache_write(k_plane, k, v_plane, v, slots, n, stream=0):
+    """k_plane, v_plane: CachePlane; k, v: TokenRows; the v side may be None."""
+    return load().hfk_cache_write(_ref(k_plane), _ref(k), _ref(v_plane), _ref(v), slots, n, stream)
+
+
+def cache_read(k_plane, k, v_plane, v, slots, n, stream=0):
+    return load().hfk_cache_read(_ref(k_plane), _ref(k), _ref(v_plane), _ref(v), slots, n, stream)
+
+
+def prompt_attention_workspace(a, n_seqs, table_width):
+    """(status, bytes)"""
+    out = ctypes.c_uint64(0)
+    return load().hfk_prompt_attention_workspace(_ref(a), n_seqs, table_width, ctypes.byref(out)), out.value
+
+
+def prompt_attention(a, block_table, n_seqs, table_width, query_starts, kv_lens, causal, workspace=0, workspace_bytes=0,
+                     stream=0):
+    return load().hfk_prompt_attention(_ref(a), block_table, n_seqs, table_width, query_starts, kv_lens,
+                                       int(bool(causal)), workspace, workspace_bytes, stream)
+
+
+def prefix_attention_workspace(a, n_prefix_blocks, table_width):
+    """(status, bytes)"""
+    out = ctypes.c_uint64(0)
+    return load().hfk_prefix_attention_workspace(_ref(a), n_prefix_blocks, table_width, ctypes.byref(out)), out.value
+
+
+def prefix_attention(a, prefix_blocks, n_prefix_blocks, prefix_len, block_table, table_width, kv_lens, workspace=0,
+                     workspace_bytes=0, stream=0):
+    return load().hfk_prefix_attention(_ref(a), prefix_blocks, n_prefix_blocks, prefix_len, block_table, table_width,
+                                       kv_lens, workspace, workspace_bytes, stream)
 
 
 def set_tuning(knob, value):

@@ -1089,6 +1089,9 @@ const char* hfk_status_string(int status) {
         case HFK_ERR_STAGING_BUSY:
             return "hfk: the library's static staging buffer is still in use by a call on another stream";
         case HFK_ERR_TABLE_MISMATCH: return "hfk: host_block_ids differs from the host column of block_pairs";
+        case HFK_ERR_BAD_TYPE: return "hfk: element type not taken here";
+        case HFK_ERR_BAD_ALIGNMENT: return "hfk: pointer or stride is not a multiple of 16 bytes";
+        case HFK_ERR_WORKSPACE_TOO_SMALL: return "hfk: workspace is smaller than the entry point needs";
         default: break;
     }
     if (status > 0) return hipGetErrorString((hipError_t)status);

@@ -1,6 +1,7 @@
 /*
- * hfk.h - C-ABI of libhfk_hip.so: KV-cache block swap, block gather and the
- * layout-converting multi-layer block transfer for AMD MI355X (gfx950).
+ * hfk.h - C-ABI of libhfk_hip.so: KV-cache block swap, block gather, the
+ * layout-converting multi-layer block transfer, writing tokens into the cache and reading
+ * them back, and attention over the cache, for AMD MI355X (gfx950).
  *
  * Every entry point
  *   - takes plain pointers and sizes (no torch types),
@@ -16,7 +17,8 @@
  * memory, or pinned host memory in its mapped (hipHostGetDevicePointer) form.
  * Host memory is read and written by the kernels directly over the PCIe link.
  *
- * The library moves bytes only; element types matter solely through their size.
+ * The swaps, gathers and transfers move bytes only; element types matter solely through
+ * their size. hfk_cache_write / _read and the attention entry points read values.
  */
 #ifndef HFK_H
 #define HFK_H
@@ -46,7 +48,10 @@ enum hfk_status {
     HFK_ERR_BAD_FLAGS = -6,    /* a flags argument has unknown bits set            */
     HFK_ERR_STAGING_TOO_SMALL = -7, /* the transfer does not fit the library's static staging buffer */
     HFK_ERR_STAGING_BUSY = -9,  /* the library's static staging buffer is in use by a call on another stream */
-    HFK_ERR_TABLE_MISMATCH = -8 /* two forms of the same block table disagree (HFK_KNOB_CHECK_HOST_COLUMN) */
+    HFK_ERR_TABLE_MISMATCH = -8, /* two forms of the same block table disagree (HFK_KNOB_CHECK_HOST_COLUMN) */
+    HFK_ERR_BAD_TYPE = -10,     /* an element type, or a combination of them, that the entry point does not take */
+    HFK_ERR_BAD_ALIGNMENT = -11, /* a pointer or stride is not a multiple of 16 bytes where it has to be */
+    HFK_ERR_WORKSPACE_TOO_SMALL = -12 /* the workspace is smaller than the entry point's _workspace() says */
 };
 
 /* HFK_VERSION_MAJOR * 1000 + HFK_VERSION_MINOR of the loaded library. */
@@ -426,6 +431,128 @@ HFK_API int hfk_gather_blocks(const void* dst_plane_ptrs, const void* src_plane_
                       uint64_t block_bytes, uint64_t src_block_stride,
                       uint64_t src_blocks, uint32_t flags, uint32_t workgroups,
                       hfk_stream_t stream);
+
+/* ---- tokens into the cache and out of it, attention over it --------------------------------- */
+
+enum hfk_type {
+    HFK_BF16 = 0,
+    HFK_FP16 = 1,
+    HFK_FP8_E4M3 = 2 /* OCP e4m3 (no infinities, largest value 448) */
+};
+
+/*
+ * One side (keys or values) of one layer's paged cache: element (block, token, head, d) at
+ * values + block * block_stride + token * token_stride + head * head_stride + d, strides in
+ * elements. [blocks][T][H][D] (the block swap's configurations) and [blocks][H][T][D] (the layers
+ * of hfk_multi_layer_block_transfer) are both of this form, and so is a plane whose blocks hold
+ * the values and, behind them, their scales, so that one block swap moves both.
+ *
+ * An HFK_FP8_E4M3 plane has one float scale per token and head, at scales + the same sum of the
+ * scale strides (in floats); a stored value v stands for v * scale. Scales are powers of two
+ * (hfk_cache_write makes them so): of a scale only the exponent is read. Other planes have
+ * scales == NULL.
+ *
+ * No counterpart in the reference, whose ops never look into a block.
+ */
+typedef struct hfk_cache_plane {
+    void* values;
+    float* scales;
+    int64_t block_stride, token_stride, head_stride;
+    int64_t scale_block_stride, scale_token_stride, scale_head_stride;
+    uint64_t blocks;
+    uint32_t block_tokens; /* T */
+    uint32_t heads;
+    uint32_t head_dim;
+    uint32_t type;         /* enum hfk_type */
+} hfk_cache_plane;
+
+/* Rows of tokens outside the cache, HFK_BF16 or HFK_FP16: element (token, head, d) at
+ * data + token * token_stride + head * head_stride + d, strides in elements. */
+typedef struct hfk_token_rows {
+    void* data;
+    int64_t token_stride, head_stride;
+    uint32_t type;
+} hfk_token_rows;
+
+/*
+ * Writes n tokens into the cache: token i goes to slot slots[i], slot s being token s % T of block
+ * s / T. A slot outside [0, blocks * T) (a padded row: -1) is skipped.
+ *   plane of the rows' type:  the values are copied.
+ *   HFK_FP8_E4M3 plane:       per token and head, with a = the largest finite |x|,
+ *       scale = the smallest power of two with a <= 448 * scale (1 if a == 0; within 2^-126 .. 2^119),
+ *       value = x / scale rounded to e4m3 to nearest even; infinities become +-448, NaN stays NaN.
+ *     A power of two makes the division, and the product on the way back, exact: the only error is
+ *     the rounding to 4 significant bits.
+ * v_plane and v may both be NULL (a cache of one latent tensor per layer); the two sides may differ
+ * in heads and head_dim. slots are device-visible; slots of one call must be distinct.
+ * Any head_dim up to 1024 and any strides; rows and planes whose pointers and strides are multiples of
+ * 16 bytes (8 for the HFK_FP8_E4M3 side) with head_dim a multiple of 8 take the vectorised path.
+ */
+HFK_API int hfk_cache_write(const hfk_cache_plane* k_plane, const hfk_token_rows* k, const hfk_cache_plane* v_plane,
+                            const hfk_token_rows* v, const int64_t* slots, uint64_t n, hfk_stream_t stream);
+
+/*
+ * The way back: row i = the token in slot slots[i], values times scale for an HFK_FP8_E4M3 plane (exact
+ * in HFK_BF16; in HFK_FP16 exact but for subnormals, and values beyond its range become its
+ * largest finite one). A slot outside the cache leaves its row untouched. Otherwise as hfk_cache_write;
+ * slots may repeat.
+ */
+HFK_API int hfk_cache_read(const hfk_cache_plane* k_plane, const hfk_token_rows* k, const hfk_cache_plane* v_plane,
+                           const hfk_token_rows* v, const int64_t* slots, uint64_t n, hfk_stream_t stream);
+
+/* Queries and results of one attention call. */
+typedef struct hfk_attention {
+    hfk_cache_plane k, v;        /* same blocks, block_tokens, heads, head_dim and type */
+    hfk_token_rows q, out;       /* n_rows tokens of q_heads heads of head_dim values, of one type */
+    float* lse;                  /* [n_rows][q_heads] natural logarithm of each row's sum of exponentials, or NULL */
+    uint64_t n_rows;
+    uint32_t q_heads;            /* a multiple of k.heads: query head h reads cache head h / (q_heads / k.heads) */
+    float scale;                 /* of the scores, positive and finite */
+} hfk_attention;
+
+/*
+ * Attention of packed prompts over the paged cache. Sequence b owns the rows
+ * [query_starts[b], query_starts[b + 1]) and the first kv_lens[b] tokens of the blocks
+ * block_table[b][0 .. table_width):
+ *   out[r, h] = sum_j w_j v[j],  w = softmax over the visible j of  scale * <q[r, h], k[j]>
+ * causal != 0: the sequence's last query sees all of its kv_lens[b] tokens, each query before it one
+ * token less; else every query sees all of them. The new tokens' keys and values are read from the cache too:
+ * write them first. A row that sees nothing gets zeros and lse = -infinity.
+ *
+ *   block_table   device int64 [n_seqs][table_width]; a token in a block outside [0, k.blocks) is not visible
+ *   query_starts  device int64 [n_seqs + 1], not decreasing; rows outside [query_starts[0],
+ *                 query_starts[n_seqs]) are left as they are. A sequence whose two entries are not in order
+ *                 or lie outside [0, n_rows] is skipped.
+ *   kv_lens       device int64 [n_seqs]; taken to lie within [0, table_width * T]
+ *   workspace     device memory of hfk_prompt_attention_workspace() bytes, 256-byte aligned (NULL if that is 0),
+ *                 written and read by this call alone until the stream has passed it
+ * Types: q and out HFK_BF16 or HFK_FP16; the cache of the same type or HFK_FP8_E4M3. Scores, statistics
+ * and sums are held in 32 bits; the weights are rounded to q's type for the second product.
+ * head_dim: a multiple of 16 up to 256. All pointers and strides multiples of 16 bytes.
+ */
+HFK_API int hfk_prompt_attention_workspace(const hfk_attention* a, uint64_t n_seqs, uint64_t table_width,
+                                           uint64_t* bytes);
+HFK_API int hfk_prompt_attention(const hfk_attention* a, const int64_t* block_table, uint64_t n_seqs,
+                                 uint64_t table_width, const int64_t* query_starts, const int64_t* kv_lens, int causal,
+                                 void* workspace, uint64_t workspace_bytes, hfk_stream_t stream);
+
+/*
+ * Attention of one token per sequence (a decoding step) for a batch whose sequences all begin with the
+ * same prefix: row b sees the prefix_len[0] tokens of prefix_blocks and then the kv_lens[b] tokens of
+ * block_table[b]. The prefix is read once for the whole batch, not once per sequence. Without a
+ * prefix (n_prefix_blocks == 0) this is the ordinary paged decoding step.
+ *
+ *   prefix_blocks device int64 [n_prefix_blocks];  prefix_len  device int64 [1], taken to lie within
+ *                 [0, n_prefix_blocks * T] (both may be NULL when n_prefix_blocks == 0)
+ *   block_table   device int64 [n_rows][table_width];  kv_lens  device int64 [n_rows]
+ * Everything else as hfk_prompt_attention.
+ */
+HFK_API int hfk_prefix_attention_workspace(const hfk_attention* a, uint64_t n_prefix_blocks, uint64_t table_width,
+                                           uint64_t* bytes);
+HFK_API int hfk_prefix_attention(const hfk_attention* a, const int64_t* prefix_blocks, uint64_t n_prefix_blocks,
+                                 const int64_t* prefix_len, const int64_t* block_table, uint64_t table_width,
+                                 const int64_t* kv_lens, void* workspace, uint64_t workspace_bytes,
+                                 hfk_stream_t stream);
 
 /*
  * Tuning knobs. Defaults are the measured best for MI355X. hfk_set_tuning changes a knob for the whole

@@ -9,6 +9,7 @@
 
 #include <cmath>
 #include <cstdint>
+#include <type_traits>
 
 #include "hfk.h"
 #include "hfk_attention_plan.h"
@@ -24,6 +25,7 @@ using hfk::u32x4;
 
 constexpr float kMinusInf = -__builtin_huge_valf();
 constexpr float kLn2 = 0.693147180559945309f;
+constexpr uint32_t kWideThreads = hfk::kWideRows * 2;     // a wave has 32 rows
 
 // One side of the cache for one call; strides in bytes (scales: in floats).
 struct CacheSide {
@@ -133,34 +135,29 @@ __device__ Tile find_tile(const AttentionArgs& a, const Walk& w, uint32_t tile) 
         if (past != 0) {
             const int at = __builtin_ctzll(past);
             t.seq = base + at;
-            t.first_token = __shfl((uint32_t)first, at);
-            t.tokens = __shfl(tokens, at);
-            t.first_row = (tile - before - (__shfl(upto, at) - __shfl(mine, at))) * ROWS;
+            t.first_token = __builtin_amdgcn_readlane((uint32_t)first, at);
+            t.tokens = __builtin_amdgcn_readlane(tokens, at);
+            t.first_row = (tile - before - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(mine, at))) * ROWS;
             t.found = true;
             return t;
         }
-        before += __shfl(upto, 63);
+        before += __builtin_amdgcn_readlane(upto, 63);
     }
     return t;
 }
 
-// LDS is laid out in pieces of 8 values (16 bytes); a row's pieces are permuted by its index so that the lanes that
-// read one column of pieces (K) or four rows of one (V) meet no bank twice.
+// Rows of K and V in LDS, bytes. Their paddings let a wave read 16 bytes of 16 consecutive keys (K), and 64 bytes of four
+// (V, through the transposing read), without two lanes meeting at a bank; every read of a lane then lies at a constant
+// distance from one address.
 template <int DP>
-__device__ uint32_t k_piece(uint32_t key, uint32_t piece) {
-    const uint32_t turn = DP == 64 ? (key >> 1) & 7u : key & 15u;
-    return key * (DP / 8) + (piece ^ turn);
-}
+constexpr uint32_t kKeyRow = DP * 2 + 16;
 template <int DP>
-__device__ uint32_t v_piece(uint32_t key, uint32_t piece) {
-    const uint32_t turn = DP == 64 ? ((key >> 1) & 1u) << 2 : ((key & 3u) << 2) | (((key >> 2) & 1u) << 1);
-    return key * (DP / 8) + (piece ^ turn);
-}
+constexpr uint32_t kValueRow = DP * 2 + 64;
 
 template <int KEYS>
-struct TileKeys {             // where the keys of one tile lie; -1: not visible
+struct TileKeys {             // where the keys of one tile lie; one that is not visible gets the cache's first token's place
     int64_t k[KEYS], v[KEYS];
-    uint64_t seen;            // bit per key
+    uint64_t seen;            // bit per visible key
 };
 template <int KEYS>
 struct TileScales {
@@ -168,25 +165,40 @@ struct TileScales {
 };
 
 // Four 16-bit rows' columns: lane i of 16 gets column i of the 4 x 16 values that the 16 lanes point at.
-__device__ u32x2 read_transposed(const u32x4* base, uint32_t byte) {
+__device__ u32x2 read_transposed(uint32_t lds_byte) {
     typedef short s16x4 __attribute__((ext_vector_type(4)));
     typedef __attribute__((address_space(3))) s16x4* Lds;
-    char* p = const_cast<char*>(reinterpret_cast<const char*>(base)) + byte;
-    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(s16x4*)p));
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)lds_byte));
+}
+__device__ u32x4 read_lds(uint32_t lds_byte) {
+    typedef __attribute__((address_space(3))) const u32x4* Lds;
+    return *(Lds)lds_byte;
+}
+__device__ uint32_t lds_address(const void* p) {
+    typedef __attribute__((address_space(3))) const void* Lds;
+    return (uint32_t)(uintptr_t)(Lds)p;
+}
+// Keeps an address as one register: what is added to it later stays a constant in the instruction, instead of one hoisted
+// register for every read of an unrolled loop.
+__device__ uint32_t one_register(uint32_t x) {
+    asm volatile("" : "+v"(x));
+    return x;
 }
 
-template <typename T, bool FP8, int DP, int WAVES, int RW, int KEYS>
-__global__ __launch_bounds__(WAVES * 64) void wide_attention_kernel(const AttentionArgs a, const Walk w) {
-    constexpr uint32_t kThreads = WAVES * 64, kRows = WAVES * RW * 32;
+template <typename T, bool FP8, int DP, int KEYS>
+__global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(const AttentionArgs a, const Walk w) {
+    constexpr uint32_t kRows = hfk::kWideRows, kThreads = kWideThreads, kWaves = kThreads / 64;
     constexpr uint32_t kPieces = FP8 ? DP / 16 : DP / 8;                  // 16-byte pieces of a cached row
     constexpr uint32_t kLoads = (KEYS * kPieces + kThreads - 1) / kThreads;
-    __shared__ u32x4 k_lds[2][KEYS * DP / 8];
-    __shared__ u32x4 v_lds[2][KEYS * DP / 8];
-    __shared__ TileKeys<KEYS> keys[3];
-    __shared__ TileScales<FP8 ? KEYS : 1> scales[3];
-    __shared__ uint32_t not_finite[3];
+    constexpr uint32_t kKeyStage = KEYS * kKeyRow<DP>, kValueStage = KEYS * kValueRow<DP>;
+    constexpr uint32_t kRing = 8;                                         // tiles whose places are kept
+    __shared__ __align__(16) char k_lds[3 * kKeyStage];
+    __shared__ __align__(16) char v_lds[3 * kValueStage];
+    __shared__ TileKeys<KEYS> keys[kRing];
+    __shared__ TileScales<FP8 ? KEYS : 1> scales[kRing];
+    __shared__ uint32_t not_finite;
 
-    const uint32_t tid = threadIdx.x, lane = tid % 64u, wave = tid / 64u, col = lane % 32u, half = lane / 32u;
+    const uint32_t tid = threadIdx.x, lane = tid % 64u, wave = __builtin_amdgcn_readfirstlane(tid / 64u), col = lane % 32u, half = lane / 32u;
     const uint32_t head = blockIdx.x % a.cache_heads, rest = blockIdx.x / a.cache_heads;
     const uint32_t split = rest % w.splits;
     const Tile t = find_tile<kRows>(a, w, w.tiles - 1u - rest / w.splits);   // long tiles of a causal walk first
@@ -212,43 +224,29 @@ __global__ __launch_bounds__(WAVES * 64) void wide_attention_kernel(const Attent
         end_key = most - first_key < span ? most : first_key + span;
     }
 
-    // This lane's query rows.
-    uint32_t token[RW], q_head[RW];
-    bool owns[RW];
-    int32_t limit[RW];
-    typename T::Vec8 q[RW][DP / 16];
-    const uint32_t wave_row = t.first_row + wave * (RW * 32u);
-    for (int r = 0; r < RW; ++r) {
-        const uint32_t row = wave_row + r * 32u + col;
-        owns[r] = row < n_tile_rows;
-        const uint32_t local = owns[r] ? row / a.group : 0u;
-        token[r] = t.first_token + local;
-        q_head[r] = head * a.group + (owns[r] ? row % a.group : 0u);
-        limit[r] = owns[r] ? seen_by(local) : 0;
-        const char* src = a.q + (int64_t)token[r] * a.q_token + (int64_t)q_head[r] * a.q_head;
+    // This lane's query row, and whether its wave has any.
+    const uint32_t wave_row = t.first_row + wave * 32u, row = wave_row + col;
+    const bool any_row = wave_row < n_tile_rows, owns = row < n_tile_rows;
+    const uint32_t local = owns ? row / a.group : 0u, token = t.first_token + local, q_head = head * a.group + (owns ? row % a.group : 0u);
+    const int32_t limit = owns ? seen_by(local) : 0;
+    typename T::Vec8 q[DP / 16];
+    {
+        const char* src = a.q + (int64_t)token * a.q_token + (int64_t)q_head * a.q_head;
         for (int s = 0; s < DP / 16; ++s) {
             const uint32_t d = s * 16u + half * 8u;
             u32x4 x{0, 0, 0, 0};
-            if (owns[r] && d < a.dim) x = *reinterpret_cast<const u32x4*>(src + 2u * d);
-            q[r][s] = as_vec8<T>(x);
+            if (owns && d < a.dim) x = *reinterpret_cast<const u32x4*>(src + 2u * d);
+            q[s] = as_vec8<T>(x);
         }
     }
-    // Of the wave: the fewest and the most keys one of its rows sees. Rows that do not exist see nothing and count for
-    // the most only.
-    const bool any_row = wave_row < n_tile_rows;
-    const uint32_t wave_last = wave_row + RW * 32u < n_tile_rows ? wave_row + RW * 32u - 1u : n_tile_rows - 1u;
+    // The fewest keys that a row of the wave, and of the tile, sees.
     const uint32_t wave_least = any_row ? (uint32_t)seen_by(wave_row / a.group) : 0u;
-    const uint32_t wave_most = any_row ? (uint32_t)seen_by(wave_last / a.group) : 0u;
     const uint32_t tile_least = (uint32_t)seen_by(t.first_row / a.group);
 
-    f32x16 o[RW][DP / 32];
-    float top[RW], sum[RW];
-    for (int r = 0; r < RW; ++r) {
-        top[r] = kMinusInf;
-        sum[r] = 0.0f;
-        for (int b = 0; b < DP / 32; ++b)
-            for (int i = 0; i < 16; ++i) o[r][b][i] = 0.0f;
-    }
+    f32x16 o[DP / 32];
+    float top = kMinusInf, sum = 0.0f;
+    for (int b = 0; b < DP / 32; ++b)
+        for (int i = 0; i < 16; ++i) o[b][i] = 0.0f;
 
     const int64_t* table = w.table + (uint64_t)t.seq * w.width;
     const char* k_base = a.k.values + (int64_t)head * a.k.head;
@@ -257,7 +255,7 @@ __global__ __launch_bounds__(WAVES * 64) void wide_attention_kernel(const Attent
     const float* v_scale_base = FP8 ? a.v.scales + (int64_t)head * a.v.scale_head : nullptr;
     const uint32_t n_tiles = (end_key - first_key + KEYS - 1u) / KEYS;
 
-    // Lane l of wave 0 looks up key l of a tile: the table entry is loaded a tile early, the place written late.
+    // Lane l of wave 0 looks up key l of a tile: the table entry is loaded early, the place written late.
     const auto load_entry = [&](uint32_t tile) -> int64_t {
         const uint32_t key = first_key + tile * KEYS + lane;
         return lane < KEYS && key < end_key ? table[a.split.block32(key)] : -1;
@@ -266,229 +264,329 @@ __global__ __launch_bounds__(WAVES * 64) void wide_attention_kernel(const Attent
         const uint32_t key = first_key + tile * KEYS + lane;
         const bool ok = (uint64_t)entry < a.blocks;
         const uint32_t at = key - a.split.block32(key) * a.split.T;
-        TileKeys<KEYS>& out = keys[tile % 3u];
+        TileKeys<KEYS>& out = keys[tile % kRing];
         if (lane < KEYS) {
-            out.k[lane] = ok ? place(a.k, (uint32_t)entry, at) : -1;
-            out.v[lane] = ok ? place(a.v, (uint32_t)entry, at) : -1;
+            out.k[lane] = ok ? place(a.k, (uint32_t)entry, at) : 0;
+            out.v[lane] = ok ? place(a.v, (uint32_t)entry, at) : 0;
             if constexpr (FP8) {
-                scales[tile % 3u].k[lane] = ok ? scale_place(a.k, (uint32_t)entry, at) : 0;
-                scales[tile % 3u].v[lane] = ok ? scale_place(a.v, (uint32_t)entry, at) : 0;
+                scales[tile % kRing].k[lane] = ok ? scale_place(a.k, (uint32_t)entry, at) : 0;
+                scales[tile % kRing].v[lane] = ok ? scale_place(a.v, (uint32_t)entry, at) : 0;
             }
         }
         const uint64_t seen = __ballot(ok);
         if (lane == 0) out.seen = seen;
     };
 
-    u32x4 k_reg[kLoads], v_reg[kLoads];
-    float k_scale[kLoads], v_scale[kLoads];
-    const auto load_tile = [&](uint32_t tile) {
-        const TileKeys<KEYS>& from = keys[tile % 3u];
+    // Which keys of a tile are visible, as a scalar.
+    constexpr uint64_t kAll = KEYS == 64 ? ~0ull : (1ull << (KEYS % 64)) - 1ull;
+    const auto as_scalar = [](uint64_t x) -> uint64_t {
+        return (uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(x >> 32)) << 32 | __builtin_amdgcn_readfirstlane((uint32_t)x);
+    };
+    // A tile's keys, or its values, into registers and from there into their stage. A thread has the same piece of every
+    // row it moves; pieces beyond head_dim stay zero.
+    struct Pieces {
+        u32x4 v[kLoads];
+        float scale[kLoads];
+    };
+    static_assert(kThreads % kPieces == 0);
+    const uint32_t piece = tid % kPieces, my_key = tid / kPieces;
+    const bool moves = piece * (FP8 ? 16u : 8u) < a.dim;
+    const auto key_of = [&](uint32_t n) { return n * (kThreads / kPieces) + my_key; };
+    Pieces k_reg, v_reg;
+    for (uint32_t n = 0; n < kLoads; ++n) {
+        k_reg.v[n] = v_reg.v[n] = u32x4{0, 0, 0, 0};
+        k_reg.scale[n] = v_reg.scale[n] = 1.0f;
+    }
+    // Places are read from LDS a turn before the loads that need them.
+    struct Places {
+        int64_t at[kLoads], scale[FP8 ? kLoads : 1];
+    };
+    Places k_place, v_place;
+    const auto read_places = [&](Places& p, const int64_t* at, const int64_t* scale) {
         for (uint32_t n = 0; n < kLoads; ++n) {
-            const uint32_t at = n * kThreads + tid, key = at / kPieces, piece = at % kPieces;
-            k_reg[n] = v_reg[n] = u32x4{0, 0, 0, 0};
-            if (KEYS * kPieces % kThreads != 0 && key >= KEYS) continue;
-            const int64_t kp = from.k[key], vp = from.v[key];
-            if (kp >= 0 && piece * (FP8 ? 16u : 8u) < a.dim) {
-                k_reg[n] = *reinterpret_cast<const u32x4*>(k_base + kp + piece * 16u);
-                v_reg[n] = *reinterpret_cast<const u32x4*>(v_base + vp + piece * 16u);
-                if constexpr (FP8) {
-                    k_scale[n] = k_scale_base[scales[tile % 3u].k[key]];
-                    v_scale[n] = v_scale_base[scales[tile % 3u].v[key]];
-                }
-            }
+            const uint32_t key = KEYS * kPieces % kThreads != 0 ? key_of(n) % KEYS : key_of(n);
+            p.at[n] = at[key];
+            if constexpr (FP8) p.scale[n] = scale[key];
         }
     };
-    // A value that is no number must not reach rows that do not see its key (0 * NaN): in tiles that some row sees in part,
-    // such values of V are taken out here, and added to the rows that do see them by add_not_finite.
-    const auto without_not_finite = [&](u32x4 v, bool& found) -> u32x4 {
-        for (int i = 0; i < 4; ++i) {
-            if ((v[i] & T::kExponent) == T::kExponent) {
-                v[i] &= 0xffff0000u;
-                found = true;
-            }
-            if (((v[i] >> 16) & T::kExponent) == T::kExponent) {
-                v[i] &= 0xffffu;
-                found = true;
-            }
-        }
-        return v;
-    };
-    const auto store_tile = [&](uint32_t tile) {
-        u32x4* ks = k_lds[tile & 1u];
-        u32x4* vs = v_lds[tile & 1u];
-        const bool partly = first_key + (tile + 1u) * KEYS > tile_least;
-        bool found = false;
+    const auto load_pieces = [&](Pieces& p, const Places& from, const char* base, const float* scale_base) {
+        if (!moves) return;
         for (uint32_t n = 0; n < kLoads; ++n) {
-            const uint32_t at = n * kThreads + tid, key = at / kPieces, piece = at % kPieces;
+            if (KEYS * kPieces % kThreads != 0 && key_of(n) >= KEYS) continue;
+            p.v[n] = *reinterpret_cast<const u32x4*>(base + from.at[n] + piece * 16u);
+            if constexpr (FP8) p.scale[n] = scale_base[from.scale[n]];
+        }
+    };
+    const auto read_k_places = [&](uint32_t tile) { read_places(k_place, keys[tile % kRing].k, scales[tile % kRing].k); };
+    const auto read_v_places = [&](uint32_t tile) { read_places(v_place, keys[tile % kRing].v, scales[tile % kRing].v); };
+    const auto load_k = [&](Pieces& to) { load_pieces(to, k_place, k_base, k_scale_base); };
+    const auto load_v = [&] { load_pieces(v_reg, v_place, v_base, v_scale_base); };
+    const auto store_pieces = [&](const Pieces& p, auto put) {
+        for (uint32_t n = 0; n < kLoads; ++n) {
+            const uint32_t key = key_of(n);
             if (KEYS * kPieces % kThreads != 0 && key >= KEYS) continue;
             if constexpr (FP8) {
                 for (int h = 0; h < 2; ++h) {
-                    const uint32_t k0 = k_reg[n][2 * h], k1 = k_reg[n][2 * h + 1], v0 = v_reg[n][2 * h], v1 = v_reg[n][2 * h + 1];
-                    const float ksc = k_scale[n], vsc = v_scale[n];
-                    ks[k_piece<DP>(key, 2 * piece + h)] =
-                        u32x4{T::template from_fp8<false>(k0, ksc), T::template from_fp8<true>(k0, ksc),
-                              T::template from_fp8<false>(k1, ksc), T::template from_fp8<true>(k1, ksc)};
-                    u32x4 v{T::template from_fp8<false>(v0, vsc), T::template from_fp8<true>(v0, vsc),
-                            T::template from_fp8<false>(v1, vsc), T::template from_fp8<true>(v1, vsc)};
-                    if (partly) v = without_not_finite(v, found);
-                    vs[v_piece<DP>(key, 2 * piece + h)] = v;
+                    const uint32_t x = p.v[n][2 * h], y = p.v[n][2 * h + 1];
+                    put(key, 2 * piece + h,
+                        u32x4{T::template from_fp8<false>(x, p.scale[n]), T::template from_fp8<true>(x, p.scale[n]),
+                              T::template from_fp8<false>(y, p.scale[n]), T::template from_fp8<true>(y, p.scale[n])});
                 }
             } else {
-                ks[k_piece<DP>(key, piece)] = k_reg[n];
-                u32x4 v = v_reg[n];
-                if (partly) v = without_not_finite(v, found);
-                vs[v_piece<DP>(key, piece)] = v;
+                put(key, piece, p.v[n]);
             }
         }
-        if (found) not_finite[tile % 3u] = 1u;
     };
-    // Rare and slow: every value of a key that is no number, to every row that sees the key.
-    const auto add_not_finite = [&](uint32_t tile) {
-        const uint32_t key0 = first_key + tile * KEYS;
-        for (uint32_t key = 0; key < KEYS; ++key) {
-            const int64_t vp = keys[tile % 3u].v[key];
-            if (vp < 0) continue;
-            const char* row = v_base + vp;
-            const float scale = FP8 ? v_scale_base[scales[tile % 3u].v[key]] : 1.0f;
-            for (int b = 0; b < DP / 32; ++b) {
-                for (int i = 0; i < 16; ++i) {
-                    const uint32_t d = b * 32 + 8 * (i / 4) + 4 * half + i % 4;
-                    if (d >= a.dim) continue;
-                    uint32_t bits;
-                    if constexpr (FP8) bits = T::template from_fp8<false>(reinterpret_cast<const uint8_t*>(row)[d], scale) & 0xffffu;
-                    else bits = reinterpret_cast<const uint16_t*>(row)[d];
-                    if ((bits & T::kExponent) != T::kExponent) continue;
-                    for (int r = 0; r < RW; ++r)
-                        if ((int32_t)(key0 + key) < limit[r]) o[r][b][i] += T::to_float(bits);
+    const auto store_k = [&](uint32_t tile, const Pieces& from) {
+        char* to = k_lds + tile % 3u * kKeyStage;
+        store_pieces(from, [&](uint32_t key, uint32_t at, u32x4 x) { *reinterpret_cast<u32x4*>(to + key * kKeyRow<DP> + at * 16u) = x; });
+    };
+    // V of a key that a row does not see meets a weight of zero there, and must be a number for that. Keys that no row sees
+    // become zeros; in tiles that some row sees in part, values that are no numbers are taken out here and given to the rows
+    // that do see them at the end.
+    const auto store_v = [&](uint32_t tile, uint64_t seen) {
+        char* to = v_lds + tile % 3u * kValueStage;
+        if (seen == kAll && first_key + (tile + 1u) * KEYS <= tile_least) {
+            store_pieces(v_reg, [&](uint32_t key, uint32_t at, u32x4 x) { *reinterpret_cast<u32x4*>(to + key * kValueRow<DP> + at * 16u) = x; });
+            return;
+        }
+        bool found = false;
+        store_pieces(v_reg, [&](uint32_t key, uint32_t at, u32x4 x) {
+            const bool visible = ((seen >> key) & 1u) != 0;
+            for (int i = 0; i < 4; ++i) {
+                if (!visible) x[i] = 0u;
+                if ((x[i] & T::kExponent) == T::kExponent) {
+                    x[i] &= 0xffff0000u;
+                    found = true;
+                }
+                if (((x[i] >> 16) & T::kExponent) == T::kExponent) {
+                    x[i] &= 0xffffu;
+                    found = true;
                 }
             }
-        }
+            *reinterpret_cast<u32x4*>(to + key * kValueRow<DP> + at * 16u) = x;
+        });
+        if (found) not_finite = 1u;
     };
 
-    if (n_tiles != 0) {
-        if (tid < 3u) not_finite[tid] = 0u;
-        if (wave == 0) {
-            put_keys(0, load_entry(0));
-            if (n_tiles > 1u) put_keys(1, load_entry(1));
+    // Where this lane reads in a stage.
+    const uint32_t k_from = lds_address(k_lds) + col * kKeyRow<DP> + half * 16u;
+    const uint32_t v_from = lds_address(v_lds) + (4 * half + (lane & 15u) / 4u) * kValueRow<DP> + (lane & 16u) * 2u + (lane & 3u) * 8u;
+
+    struct Scores {
+        f32x16 s[KEYS / 32];
+    };
+    struct Weights {
+        typename T::Vec8 p[KEYS / 16];
+    };
+    Scores x;
+    Weights y;
+    const auto first_product = [&](uint32_t tile) {
+        for (int b = 0; b < KEYS / 32; ++b)
+            for (int i = 0; i < 16; ++i) x.s[b][i] = 0.0f;
+        const uint32_t from = one_register(k_from + tile % 3u * kKeyStage);
+        for (int d = 0; d < DP / 16; ++d)
+            for (int b = 0; b < KEYS / 32; ++b)
+                x.s[b] = T::mfma32(as_vec8<T>(read_lds(from + (b * 32u * kKeyRow<DP> + d * 32u))), q[d], x.s[b]);
+    };
+    const auto hide = [&](uint32_t tile, uint64_t seen) {
+        const uint32_t key0 = first_key + tile * KEYS;
+        if (key0 + KEYS > wave_least) {
+            asm volatile("");      // a branch that most tiles take past all of this, no selects
+            const int32_t mine = limit - (int32_t)(key0 + 4u * half);
+            for (int b = 0; b < KEYS / 32; ++b)
+                for (int i = 0; i < 16; ++i) x.s[b][i] = b * 32 + 8 * (i / 4) + i % 4 < mine ? x.s[b][i] : kMinusInf;
         }
-        __syncthreads();
-        load_tile(0);
-        store_tile(0);
-        __syncthreads();
-    }
+        if (seen != kAll) {
+            asm volatile("");
+            for (int b = 0; b < KEYS / 32; ++b) {
+                const uint32_t mine = (uint32_t)(seen >> (32 * b)) >> (4u * half);
+                for (int i = 0; i < 16; ++i) x.s[b][i] = (mine & (1u << (8 * (i / 4) + i % 4))) != 0 ? x.s[b][i] : kMinusInf;
+            }
+        }
+    };
     // The running maximum moves when a score passes it by 2^8, so that most tiles spare the accumulator's rescaling.
     constexpr float kLazily = 8.0f, kLift = T::kMostWeight != 0.0f ? T::kMostWeight - kLazily : 0.0f;
     const float lazily = kLazily / a.score_scale;
-    for (uint32_t tile = 0; tile < n_tiles; ++tile) {
-        const uint32_t key0 = first_key + tile * KEYS;
-        const bool more = tile + 1u < n_tiles, yet_more = tile + 2u < n_tiles;
-        int64_t entry = -1;
-        if (yet_more && wave == 0) entry = load_entry(tile + 2u);
-        if (more) load_tile(tile + 1u);
-
-        if (key0 < wave_most) {
-            const u32x4* ks = k_lds[tile & 1u];
-            const u32x4* vs = v_lds[tile & 1u];
-            f32x16 s[RW][KEYS / 32];
-            for (int r = 0; r < RW; ++r)
-                for (int b = 0; b < KEYS / 32; ++b)
-                    for (int i = 0; i < 16; ++i) s[r][b][i] = 0.0f;
-            for (int b = 0; b < KEYS / 32; ++b)
-                for (int d = 0; d < DP / 16; ++d) {
-                    const auto kf = as_vec8<T>(ks[k_piece<DP>(b * 32 + col, d * 2 + half)]);
-                    for (int r = 0; r < RW; ++r) s[r][b] = T::mfma32(kf, q[r][d], s[r][b]);
-                }
-            const uint64_t seen = keys[tile % 3u].seen;
-            const bool all = seen == (KEYS == 64 ? ~0ull : (1ull << (KEYS % 64)) - 1ull);
-            if (!all || key0 + KEYS > wave_least) {
-                for (int r = 0; r < RW; ++r)
-                    for (int b = 0; b < KEYS / 32; ++b)
-                        for (int i = 0; i < 16; ++i) {
-                            const uint32_t key = b * 32 + 8 * (i / 4) + 4 * half + i % 4;
-                            const bool visible = ((seen >> key) & 1ull) != 0 && (int32_t)(key0 + key) < limit[r];
-                            s[r][b][i] = visible ? s[r][b][i] : kMinusInf;
-                        }
-            }
-            typename T::Vec8 p[RW][KEYS / 16];
-            for (int r = 0; r < RW; ++r) {
-                float high = s[r][0][0];
-                for (int b = 0; b < KEYS / 32; ++b)
-                    for (int i = 0; i < 16; ++i) high = fmaxf(high, s[r][b][i]);
-                high = max_across_32(high);
-                if (__any(high > top[r] + lazily)) {
-                    const float now = fmaxf(top[r], high);
-                    const float keep = now == kMinusInf ? 1.0f : __builtin_amdgcn_exp2f((top[r] - now) * a.score_scale);
-                    top[r] = now;
-                    sum[r] *= keep;
-                    for (int b = 0; b < DP / 32; ++b)
-                        for (int i = 0; i < 16; ++i) o[r][b][i] *= keep;
-                }
-                const float base = top[r] == kMinusInf ? 0.0f : top[r] * a.score_scale - kLift;
-                float add = 0.0f;
-                for (int b = 0; b < KEYS / 32; ++b)
-                    for (int h = 0; h < 2; ++h) {
-                        float e[8];
-                        for (int i = 0; i < 8; ++i) {
-                            e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][b][8 * h + i], a.score_scale, -base));
-                            add += e[i];
-                        }
-                        p[r][2 * b + h] = as_vec8<T>(u32x4{T::pack2(e[0], e[1]), T::pack2(e[2], e[3]), T::pack2(e[4], e[5]), T::pack2(e[6], e[7])});
-                    }
-                sum[r] += add;
-            }
-            // Key order of the second product: value j of half h of 16 keys is key (j / 4) * 8 + 4 h + j % 4, as the
-            // first product's result registers have it.
-            for (int n = 0; n < KEYS / 16; ++n)
-                for (int b = 0; b < DP / 32; ++b) {
-                    const uint32_t d = b * 32 + (lane & 16u) + (lane & 3u) * 4u;
-                    const uint32_t key = n * 16 + 4 * half + (lane & 15u) / 4u;
-                    const u32x2 low = read_transposed(vs, v_piece<DP>(key, d / 8u) * 16u + (d & 4u) * 2u);
-                    const u32x2 high = read_transposed(vs, v_piece<DP>(key + 8u, d / 8u) * 16u + (d & 4u) * 2u);
-                    const auto vf = as_vec8<T>(u32x4{low[0], low[1], high[0], high[1]});
-                    for (int r = 0; r < RW; ++r) o[r][b] = T::mfma32(vf, p[r][n], o[r][b]);
-                }
-            if (not_finite[tile % 3u] != 0) add_not_finite(tile);
+    const auto raise = [&]() {
+        float high = x.s[0][0];
+        for (int b = 0; b < KEYS / 32; ++b)
+            for (int i = 0; i < 16; ++i) high = fmaxf(high, x.s[b][i]);
+        high = max_across_32(high);
+        if (__any(high > top + lazily)) {
+            const float now = fmaxf(top, high);
+            const float keep = now == kMinusInf ? 1.0f : __builtin_amdgcn_exp2f((top - now) * a.score_scale);
+            top = now;
+            sum *= keep;
+            for (int b = 0; b < DP / 32; ++b)
+                for (int i = 0; i < 16; ++i) o[b][i] *= keep;
         }
-        // What the next two tiles are put into was last read before the barrier that ended the round before this one.
-        if (tid == 0) not_finite[(tile + 2u) % 3u] = 0u;
-        if (more) store_tile(tile + 1u);
-        if (yet_more && wave == 0) put_keys(tile + 2u, entry);
+    };
+    const auto weigh = [&]() {
+        const float base = top == kMinusInf ? 0.0f : top * a.score_scale - kLift;
+        float add = 0.0f;
+        for (int b = 0; b < KEYS / 32; ++b)
+            for (int h = 0; h < 2; ++h) {
+                float e[8];
+                for (int i = 0; i < 8; ++i) {
+                    e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x.s[b][8 * h + i], a.score_scale, -base));
+                    add += e[i];
+                }
+                y.p[2 * b + h] = as_vec8<T>(u32x4{T::pack2(e[0], e[1]), T::pack2(e[2], e[3]), T::pack2(e[4], e[5]), T::pack2(e[6], e[7])});
+            }
+        sum += add;
+    };
+    // Key order of the second product: value j of half h of 16 keys is key (j / 4) * 8 + 4 h + j % 4, as the first
+    // product's result registers have it.
+    // Its first operands are read a turn early.
+    constexpr int kAhead = 6, kSteps = KEYS * DP / 512;
+    typename T::Vec8 ahead[kAhead];
+    const auto value_columns = [&](uint32_t from, int step) -> typename T::Vec8 {
+        const uint32_t at = from + (step / (DP / 32) * 16u * kValueRow<DP> + step % (DP / 32) * 64u);
+        const u32x2 low = read_transposed(at), high = read_transposed(at + 8u * kValueRow<DP>);
+        return as_vec8<T>(u32x4{low[0], low[1], high[0], high[1]});
+    };
+    const auto read_ahead = [&](uint32_t tile) {
+        const uint32_t from = one_register(v_from + tile % 3u * kValueStage);
+        for (int step = 0; step < kAhead; ++step) ahead[step] = value_columns(from, step);
+    };
+    const auto second_product = [&](uint32_t tile) {
+        const uint32_t from = one_register(v_from + tile % 3u * kValueStage);
+        for (int step = 0; step < kSteps; ++step) {
+            const int b = step % (DP / 32);
+            o[b] = T::mfma32(step < kAhead ? ahead[step] : value_columns(from, step), y.p[step / (DP / 32)], o[b]);
+        }
+    };
+
+    // The waves of a compute unit's four SIMDs come in two halves that take turns: while one half feeds the matrix units
+    // (second product of tile i - 1, first product of tile i) the other takes weights on the vector units and moves tiles,
+    // then a barrier swaps them. The second half starts one barrier late. A tile is put into its stage by both halves'
+    // threads one turn before the first half reads it; the stage, one of three, was last read two turns earlier.
+    if (tid == 0) not_finite = 0u;
+    if (n_tiles != 0) {
+        const bool late = wave >= kWaves / 2;
+        if (wave == 0) {      // tiles behind the last show nothing
+            int64_t first[6];
+            for (uint32_t i = 0; i < 6u; ++i) first[i] = load_entry(i);
+            for (uint32_t i = 0; i < 6u; ++i) put_keys(i, first[i]);
+        }
+        int64_t entry = wave == 0 ? load_entry(6u) : -1;
+        __syncthreads();      // not_finite is cleared, too
+        uint64_t seen = as_scalar(keys[0].seen), next_seen = keys[1].seen;
+        {
+            Pieces k_second = k_reg;
+            read_k_places(0);
+            read_v_places(0);
+            load_k(k_reg);
+            load_v();
+            read_k_places(1);
+            load_k(k_second);
+            store_k(0, k_reg);
+            store_v(0, seen);
+            store_k(1, k_second);
+        }
+        read_k_places(2);
+        read_v_places(1);
+        load_k(k_reg);
+        load_v();
+        read_k_places(3);
+        read_v_places(2);
         __syncthreads();
+        if (late) __syncthreads();
+        const auto vector_turn = [&](uint32_t tile) {
+            const uint64_t coming = as_scalar(next_seen);
+            store_k(tile + 2u, k_reg);
+            store_v(tile + 1u, coming);
+            // (the look-up's result before the loads are issued: a wait for it would be one for them)
+            if (wave == 0) put_keys(tile + 6u, entry);
+            load_k(k_reg);
+            if (any_row) {
+                hide(tile, seen);
+                raise();
+                read_ahead(tile);
+            }
+            load_v();
+            if (wave == 0) entry = load_entry(tile + 7u);
+            read_k_places(tile + 4u);
+            read_v_places(tile + 3u);
+            next_seen = keys[(tile + 2u) % kRing].seen;
+            if (any_row) weigh();
+            seen = coming;
+        };
+        if (any_row) first_product(0);
+        __syncthreads();
+        vector_turn(0);
+        __syncthreads();
+        for (uint32_t tile = 1; tile < n_tiles; ++tile) {
+            if (any_row) {
+                second_product(tile - 1u);
+                first_product(tile);
+            }
+            __syncthreads();
+            vector_turn(tile);
+            __syncthreads();
+        }
+        if (any_row) second_product(n_tiles - 1u);
+        if (!late) __syncthreads();
     }
 
-    for (int r = 0; r < RW; ++r) {
-        const float total = sum_across_32(sum[r]);
-        if (!owns[r]) continue;
-        const uint64_t row = (uint64_t)token[r] * (a.cache_heads * a.group) + q_head[r];
-        const float high = top[r] == kMinusInf ? kMinusInf : top[r] * a.score_scale - kLift;
+    const float total = sum_across_32(sum);
+    const uint64_t heads = a.cache_heads * a.group;
+    if (owns) {
+        const uint64_t place = (uint64_t)token * heads + q_head;
+        const float high = top == kMinusInf ? kMinusInf : top * a.score_scale - kLift;
         if (a.part_sum != nullptr) {
-            const uint64_t at = (uint64_t)(w.first_split + split) * a.n_rows * (a.cache_heads * a.group) + row;
+            const uint64_t at = (uint64_t)(w.first_split + split) * a.n_rows * heads + place;
             if (half == 0) {
                 a.part_stat[2 * at] = high;
                 a.part_stat[2 * at + 1] = total;
             }
-            if (top[r] != kMinusInf) {
+            if (top != kMinusInf) {
                 float* dst = a.part_sum + at * a.dim;
                 for (int b = 0; b < DP / 32; ++b)
                     for (int i = 0; i < 4; ++i) {
                         const uint32_t d = b * 32 + 8 * i + 4 * half;
-                        if (d < a.dim)
-                            *reinterpret_cast<f32x4*>(dst + d) = f32x4{o[r][b][4 * i], o[r][b][4 * i + 1], o[r][b][4 * i + 2], o[r][b][4 * i + 3]};
+                        if (d < a.dim) *reinterpret_cast<f32x4*>(dst + d) = f32x4{o[b][4 * i], o[b][4 * i + 1], o[b][4 * i + 2], o[b][4 * i + 3]};
                     }
             }
         } else {
-            const float inverse = top[r] == kMinusInf ? 0.0f : 1.0f / total;
-            char* dst = a.out + (int64_t)token[r] * a.out_token + (int64_t)q_head[r] * a.out_head;
+            const float inverse = top == kMinusInf ? 0.0f : 1.0f / total;
+            char* dst = a.out + (int64_t)token * a.out_token + (int64_t)q_head * a.out_head;
             for (int b = 0; b < DP / 32; ++b)
                 for (int i = 0; i < 4; ++i) {
                     const uint32_t d = b * 32 + 8 * i + 4 * half;
                     if (d < a.dim)
-                        *reinterpret_cast<u32x2*>(dst + 2u * d) =
-                            u32x2{T::pack2(o[r][b][4 * i] * inverse, o[r][b][4 * i + 1] * inverse),
-                                  T::pack2(o[r][b][4 * i + 2] * inverse, o[r][b][4 * i + 3] * inverse)};
+                        *reinterpret_cast<u32x2*>(dst + 2u * d) = u32x2{T::pack2(o[b][4 * i] * inverse, o[b][4 * i + 1] * inverse),
+                                                                      T::pack2(o[b][4 * i + 2] * inverse, o[b][4 * i + 3] * inverse)};
                 }
-            if (a.lse != nullptr && half == 0) a.lse[row] = top[r] == kMinusInf ? kMinusInf : (high + __log2f(total)) * kLn2;
+            if (a.lse != nullptr && half == 0) a.lse[place] = top == kMinusInf ? kMinusInf : (high + __log2f(total)) * kLn2;
         }
+    }
+
+    // Rare and slow: what was taken out of V, to every row that sees the key it belongs to.
+    __syncthreads();
+    if (n_tiles == 0 || not_finite == 0) return;
+    const uint32_t whole = tile_least > first_key ? (tile_least - first_key) / KEYS * KEYS : 0u;    // keys of untouched tiles
+    for (uint32_t n = tid; n < kRows * a.dim; n += kThreads) {
+        const uint32_t r = t.first_row + n / a.dim, d = n % a.dim;
+        if (r >= n_tile_rows) break;
+        const uint32_t of = r / a.group, of_head = head * a.group + r % a.group;
+        const uint32_t until = (uint32_t)seen_by(of) < end_key ? (uint32_t)seen_by(of) : end_key;
+        float add = 0.0f;
+        for (uint32_t key = first_key + whole; key < until; ++key) {
+            const uint32_t block = a.split.block32(key), at = key - block * a.split.T;
+            const int64_t entry = table[block];
+            if ((uint64_t)entry >= a.blocks) continue;
+            const char* src = v_base + place(a.v, (uint32_t)entry, at);
+            uint32_t bits;
+            if constexpr (FP8) bits = T::template from_fp8<false>(reinterpret_cast<const uint8_t*>(src)[d], v_scale_base[scale_place(a.v, (uint32_t)entry, at)]) & 0xffffu;
+            else bits = reinterpret_cast<const uint16_t*>(src)[d];
+            if ((bits & T::kExponent) == T::kExponent) add += T::to_float(bits);
+        }
+        if (add == 0.0f) continue;
+        const uint64_t at_token = t.first_token + of;
+        if (a.part_sum != nullptr) a.part_sum[((uint64_t)(w.first_split + split) * a.n_rows * heads + at_token * heads + of_head) * a.dim + d] = add;
+        else reinterpret_cast<uint16_t*>(a.out + (int64_t)at_token * a.out_token + (int64_t)of_head * a.out_head)[d] = (uint16_t)T::pack2(add, add);
     }
 }
 
@@ -860,9 +958,9 @@ int check_workspace(void* workspace, uint64_t bytes, uint64_t needed) {
 template <typename T, bool FP8>
 void launch_wide(const AttentionArgs& x, const Walk& w, hipStream_t s) {
     switch (hfk::padded_head_dim(x.dim)) {
-        case 64: wide_attention_kernel<T, FP8, 64, 4, 1, 64><<<w.groups, 256, 0, s>>>(x, w); break;
-        case 128: wide_attention_kernel<T, FP8, 128, 4, 1, 64><<<w.groups, 256, 0, s>>>(x, w); break;
-        default: wide_attention_kernel<T, FP8, 256, 4, 1, 32><<<w.groups, 256, 0, s>>>(x, w); break;
+        case 64: wide_attention_kernel<T, FP8, 64, 64><<<w.groups, kWideThreads, 0, s>>>(x, w); break;
+        case 128: wide_attention_kernel<T, FP8, 128, 64><<<w.groups, kWideThreads, 0, s>>>(x, w); break;
+        default: wide_attention_kernel<T, FP8, 256, 32><<<w.groups, kWideThreads, 0, s>>>(x, w); break;
     }
 }
 

@@ -10,7 +10,7 @@
 
 namespace hfk {
 
-constexpr uint32_t kWideRows = 128;        // query rows of a wide workgroup
+constexpr uint32_t kWideRows = 256;        // query rows of a wide workgroup
 constexpr uint32_t kMinSplitKeys = 256;    // no split shorter than this: its fixed cost would show
 
 inline uint64_t ceil_div(uint64_t a, uint64_t b) { return (a + b - 1) / b; }

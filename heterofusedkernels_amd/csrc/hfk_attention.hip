@@ -27,12 +27,14 @@ constexpr float kMinusInf = -__builtin_huge_valf();
 constexpr float kLn2 = 0.693147180559945309f;
 constexpr uint32_t kWideThreads = hfk::kWideRows * 2;     // a wave has 32 rows
 
-// One side of the cache for one call; strides in bytes (scales: in floats).
+// One side of the cache for one call; strides in bytes (scales: in floats). A block spans less than 4 GiB (checked on the
+// host), so that a token's place takes 32-bit products; only their sum over blocks is longer.
 struct CacheSide {
     const char* values;
     const float* scales;
-    int64_t block, token, head;
-    int64_t scale_block, scale_token, scale_head;
+    int64_t head, scale_head;
+    uint32_t block, token;
+    uint32_t scale_block, scale_token;
 };
 
 struct AttentionArgs {
@@ -46,22 +48,43 @@ struct AttentionArgs {
     uint32_t n_rows;          // tokens
     uint32_t cache_heads, group, dim;
     float score_scale;        // scale * log2 e
-    float* part_sum;          // NULL: the one split writes the result itself
-    float* part_stat;         // largest score, sum of weights
 };
 
-// What one launch walks: sequences of query rows with their keys.
-struct Walk {
+// Where a launch leaves what the join takes: unnormalised sums [splits][rows][dim], and beside them [splits][rows] pairs of the
+// largest score (times log2 e) and the sum of weights. A largest score of -infinity: nothing was seen, no sum was written.
+struct Partials {
+    float* sum;               // NULL: the one split writes the result itself
+    float* stat;
+};
+
+// What a wide launch walks: sequences of query rows with their keys.
+struct WideWalk {
     const int64_t* table;     // [n_seqs][width]
     uint32_t width;
-    const int64_t* starts;    // [n_seqs + 1], or NULL: sequence b owns `tokens_per_seq` tokens from b * tokens_per_seq
+    const int64_t* starts;    // [n_seqs + 1], or NULL: one sequence that owns all rows
+    const int64_t* lens;
+    uint32_t n_seqs;
+    uint32_t causal;
+    uint32_t tiles;           // of query rows, all sequences'
+    uint32_t splits;
+    uint32_t groups;          // workgroups
+    Partials to;
+};
+
+// What a narrow launch walks: the keys of n_seqs sequences as one row of units, cut into `ranges` equal shares whatever
+// sequences they fall into. Every sequence has tokens_per_seq tokens. A share's part of a sequence is a split.
+struct NarrowWalk {
+    const int64_t* table;     // [n_seqs][width]
+    uint32_t width;
     const int64_t* lens;
     uint32_t n_seqs, tokens_per_seq;
-    uint32_t causal;
-    uint32_t tiles;           // of query rows: all sequences' (wide), or per sequence (narrow)
-    uint32_t splits, chunk;   // chunk: keys per split (narrow)
-    uint32_t first_split;     // place of split 0 in the workspace
+    uint32_t tiles;           // of query rows, per sequence
+    uint32_t unit;            // keys: 32 for each wave that works at one head
+    uint32_t ranges;
     uint32_t groups;          // workgroups
+    // n_seqs == 1: split s is range s and has every row. Else range g's part of sequence b is split g + b, which no other
+    // part is (from one part to the next at least one of the two grows), and has b's rows alone.
+    Partials to;
 };
 
 __device__ uint32_t clamp_len(int64_t len, uint32_t width, uint32_t T) {
@@ -87,14 +110,20 @@ __device__ float sum_across_16(float x) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// The running maximum moves when a score passes it by 2^8, so that most tiles spare the accumulator's rescaling.
+constexpr float kLazily = 8.0f;
+// Weights of the type T are lifted so that none passes 2^kMostWeight.
+template <typename T>
+constexpr float kLiftOf = T::kMostWeight != 0.0f ? T::kMostWeight - kLazily : 0.0f;
+
 template <typename T, typename V>
 __device__ typename T::Vec8 as_vec8(V v) {
     return __builtin_bit_cast(typename T::Vec8, v);
 }
 
-__device__ int64_t place(const CacheSide& s, uint32_t block, uint32_t at) { return (int64_t)block * s.block + (int64_t)at * s.token; }
+__device__ int64_t place(const CacheSide& s, uint32_t block, uint32_t at) { return (int64_t)((uint64_t)block * s.block + at * s.token); }
 __device__ int64_t scale_place(const CacheSide& s, uint32_t block, uint32_t at) {
-    return (int64_t)block * s.scale_block + (int64_t)at * s.scale_token;
+    return (int64_t)((uint64_t)block * s.scale_block + at * s.scale_token);
 }
 
 // ---- wide -------------------------------------------------------------------------------------
@@ -106,10 +135,10 @@ struct Tile {
 };
 
 template <uint32_t ROWS>
-__device__ Tile find_tile(const AttentionArgs& a, const Walk& w, uint32_t tile) {
+__device__ Tile find_tile(const AttentionArgs& a, const WideWalk& w, uint32_t tile) {
     Tile t{0, 0, 0, 0, false};
     if (w.starts == nullptr) {
-        t.tokens = w.tokens_per_seq;
+        t.tokens = a.n_rows;
         t.first_row = tile * ROWS;
         t.found = t.first_row < t.tokens * a.group;
         return t;
@@ -186,7 +215,7 @@ __device__ uint32_t one_register(uint32_t x) {
 }
 
 template <typename T, bool FP8, int DP, int KEYS>
-__global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(const AttentionArgs a, const Walk w) {
+__global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(const AttentionArgs a, const WideWalk w) {
     constexpr uint32_t kRows = hfk::kWideRows, kThreads = kWideThreads, kWaves = kThreads / 64;
     constexpr uint32_t kPieces = FP8 ? DP / 16 : DP / 8;                  // 16-byte pieces of a cached row
     constexpr uint32_t kLoads = (KEYS * kPieces + kThreads - 1) / kThreads;
@@ -405,8 +434,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(const A
             }
         }
     };
-    // The running maximum moves when a score passes it by 2^8, so that most tiles spare the accumulator's rescaling.
-    constexpr float kLazily = 8.0f, kLift = T::kMostWeight != 0.0f ? T::kMostWeight - kLazily : 0.0f;
+    constexpr float kLift = kLiftOf<T>;
     const float lazily = kLazily / a.score_scale;
     const auto raise = [&]() {
         float high = x.s[0][0];
@@ -535,14 +563,14 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(const A
     if (owns) {
         const uint64_t place = (uint64_t)token * heads + q_head;
         const float high = top == kMinusInf ? kMinusInf : top * a.score_scale - kLift;
-        if (a.part_sum != nullptr) {
-            const uint64_t at = (uint64_t)(w.first_split + split) * a.n_rows * heads + place;
+        if (w.to.sum != nullptr) {
+            const uint64_t at = (uint64_t)split * a.n_rows * heads + place;
             if (half == 0) {
-                a.part_stat[2 * at] = high;
-                a.part_stat[2 * at + 1] = total;
+                w.to.stat[2 * at] = high;
+                w.to.stat[2 * at + 1] = total;
             }
             if (top != kMinusInf) {
-                float* dst = a.part_sum + at * a.dim;
+                float* dst = w.to.sum + at * a.dim;
                 for (int b = 0; b < DP / 32; ++b)
                     for (int i = 0; i < 4; ++i) {
                         const uint32_t d = b * 32 + 8 * i + 4 * half;
@@ -585,306 +613,474 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(const A
         }
         if (add == 0.0f) continue;
         const uint64_t at_token = t.first_token + of;
-        if (a.part_sum != nullptr) a.part_sum[((uint64_t)(w.first_split + split) * a.n_rows * heads + at_token * heads + of_head) * a.dim + d] = add;
+        if (w.to.sum != nullptr) w.to.sum[((uint64_t)split * a.n_rows * heads + at_token * heads + of_head) * a.dim + d] = add;
         else reinterpret_cast<uint16_t*>(a.out + (int64_t)at_token * a.out_token + (int64_t)of_head * a.out_head)[d] = (uint16_t)T::pack2(add, add);
     }
 }
 
 // ---- narrow -----------------------------------------------------------------------------------
 
-template <typename T, bool FP8, int DP, int R>
-__global__ __launch_bounds__(256) void narrow_attention_kernel(const AttentionArgs a, const Walk prefix, const Walk own) {
+__device__ uint32_t units_of(const NarrowWalk& w, uint32_t T, uint32_t seq) {
+    return (clamp_len(w.lens[seq], w.width, T) + w.unit - 1u) / w.unit;
+}
+
+// Units of all sequences, and of those before `seq`. By every wave alike, 64 sequences at a time.
+struct UnitSums {
+    uint32_t all, before;
+};
+__device__ UnitSums sum_units(const NarrowWalk& w, uint32_t T, uint32_t seq) {
+    const uint32_t lane = threadIdx.x % 64u;
+    uint32_t all = 0, before = 0;
+    for (uint32_t b = lane; b < w.n_seqs; b += 64u) {
+        const uint32_t n = units_of(w, T, b);
+        all += n;
+        before += b < seq ? n : 0u;
+    }
+    for (uint32_t o = 32; o != 0; o >>= 1) {
+        all += __shfl_xor(all, (int)o);
+        before += __shfl_xor(before, (int)o);
+    }
+    return {(uint32_t)__builtin_amdgcn_readfirstlane(all), (uint32_t)__builtin_amdgcn_readfirstlane(before)};
+}
+__device__ uint32_t share_of(const NarrowWalk& w, uint32_t all) {
+    const uint32_t n = (all + w.ranges - 1u) / w.ranges;
+    return n == 0 ? 1u : n;
+}
+
+// The sequence that unit `unit` is in, and its first unit. There is one: unit < all.
+struct UnitPlace {
+    uint32_t seq, start;
+};
+__device__ UnitPlace find_unit(const NarrowWalk& w, uint32_t T, uint32_t unit) {
+    const uint32_t lane = threadIdx.x % 64u;
+    uint32_t before = 0;
+    for (uint32_t base = 0; base < w.n_seqs; base += 64u) {
+        const uint32_t b = base + lane, mine = b < w.n_seqs ? units_of(w, T, b) : 0u;
+        uint32_t upto = mine;
+        for (uint32_t o = 1; o < 64u; o <<= 1) {
+            const uint32_t other = __shfl_up(upto, o);
+            if (lane >= o) upto += other;
+        }
+        const uint64_t past = __ballot(before + upto > unit);
+        if (past != 0) {
+            const int at = __builtin_ctzll(past);
+            return {base + at, before + (uint32_t)__builtin_amdgcn_readlane(upto, at) - (uint32_t)__builtin_amdgcn_readlane(mine, at)};
+        }
+        before += __builtin_amdgcn_readlane(upto, 63);
+    }
+    return {w.n_seqs, before};
+}
+
+// HEADS == 4: a wave for each of four neighbouring cache heads, all at the same keys. HEADS == 1: four waves at one head, whose
+// sums meet in LDS.
+template <typename T, bool FP8, int DP, int R, int HEADS>
+__global__ __launch_bounds__(256, R * DP <= 256 ? 2 : 1) void narrow_attention_kernel(const AttentionArgs a, const NarrowWalk prefix, const NarrowWalk own) {
     constexpr int kKSteps = DP / 32;        // matrix instructions of the first product
     constexpr int kCols = DP / 16;          // values of V per lane and key
-    constexpr uint32_t kRegs = R * kCols * 4;
-    constexpr float kLift = T::kMostWeight;
-    __shared__ float tops[4][R * 16], sums[4][R * 16];
-    __shared__ float o_lds[2][kRegs * 64];
-
-    const uint32_t tid = threadIdx.x, lane = tid % 64u, wave = tid / 64u, col = lane % 16u, quarter = lane / 16u;
-    const bool is_prefix = blockIdx.x < prefix.groups;
-    const Walk& w = is_prefix ? prefix : own;
-    const uint32_t group_id = is_prefix ? blockIdx.x : blockIdx.x - prefix.groups;
-    const uint32_t head = group_id % a.cache_heads, rest = group_id / a.cache_heads;
-    const uint32_t split = rest % w.splits, tile = rest / w.splits % w.tiles, seq = rest / w.splits / w.tiles;
-
-    const uint32_t len = clamp_len(w.lens[seq], w.width, a.split.T);
-    const uint64_t from = (uint64_t)split * w.chunk;
-    const uint32_t first_key = from < len ? (uint32_t)from : len;
-    const uint32_t end_key = len - first_key < w.chunk ? len : first_key + w.chunk;
-    const uint32_t n_tile_rows = w.tokens_per_seq * a.group;
-
-    uint32_t token[R], q_head[R];
-    bool owns[R];
-    typename T::Vec8 q[R][kKSteps];
-    for (int r = 0; r < R; ++r) {
-        const uint32_t row = (tile * R + r) * 16u + col;
-        owns[r] = row < n_tile_rows;
-        token[r] = seq * w.tokens_per_seq + (owns[r] ? row / a.group : 0u);
-        q_head[r] = head * a.group + (owns[r] ? row % a.group : 0u);
-        const char* src = a.q + (int64_t)token[r] * a.q_token + (int64_t)q_head[r] * a.q_head;
-        for (int s = 0; s < kKSteps; ++s) {
-            // an e4m3 row is loaded 16 values at a time, which two steps share
-            const uint32_t d = FP8 ? (s / 2) * 64u + quarter * 16u + (s % 2) * 8u : s * 32u + quarter * 8u;
-            u32x4 x{0, 0, 0, 0};
-            if (owns[r] && d < a.dim) x = *reinterpret_cast<const u32x4*>(src + 2u * d);
-            q[r][s] = as_vec8<T>(x);
-        }
-    }
-    f32x4 o[R][kCols];
-    float top[R], sum[R];
-    for (int r = 0; r < R; ++r) {
-        top[r] = kMinusInf;
-        sum[r] = 0.0f;
-        for (int c = 0; c < kCols; ++c) o[r][c] = f32x4{0, 0, 0, 0};
-    }
-
-    const int64_t* table = w.table + (uint64_t)seq * w.width;
-    const char* k_base = a.k.values + (int64_t)head * a.k.head;
-    const char* v_base = a.v.values + (int64_t)head * a.v.head;
-    const float* k_scale_base = FP8 ? a.k.scales + (int64_t)head * a.k.scale_head : nullptr;
-    const float* v_scale_base = FP8 ? a.v.scales + (int64_t)head * a.v.scale_head : nullptr;
-    // One block for four keys in a row when blocks hold a multiple of four.
-    const bool by_four = a.split.T % 4u == 0;
-
-    const auto look_up = [&](uint32_t key, uint32_t& block, uint32_t& at) -> bool {
-        block = at = 0;
-        if (key >= end_key) return false;
-        const uint32_t n = a.split.block32(key);
-        const int64_t entry = table[n];
-        if ((uint64_t)entry >= a.blocks) return false;
-        block = (uint32_t)entry;
-        at = key - n * a.split.T;
-        return true;
+    constexpr uint32_t kRegs = R * kCols * 4, kWavesPerHead = 4 / HEADS, kUnit = kWavesPerHead * 32;
+    constexpr int kRowPieces = FP8 ? DP / 16 : DP / 8;                   // 16-byte pieces of a cached row
+    constexpr uint32_t kRowBytes = kRowPieces * 16 + 16;                 // of K in LDS: 16 rows' pieces of one column, no bank twice
+    struct WaveLds {                                                     // a wave's own: no barrier, LDS serves a wave in order
+        char k[32 * kRowBytes];
+        int64_t place[32][2];                                            // of a key's K and V
+        float scale[2][FP8 ? 32 : 1];
     };
+    __shared__ float tops[4][R * 16], sums[4][R * 16];
+    __shared__ __align__(16) union {
+        WaveLds wave[4];
+        float o[2][HEADS == 1 ? kRegs * 64 : 1];                         // once the keys are done
+    } lds;
 
-    for (uint32_t key0 = first_key + wave * 32u; key0 < end_key; key0 += 128u) {
-        // The first product's keys: 16 t + col. A lane without its key reads the cache's first row instead and its scores are
-        // masked.
-        u32x4 k_reg[2][FP8 ? DP / 64 : DP / 32];
-        float k_scale[2];
-        uint32_t seen = 0;
-        for (int t = 0; t < 2; ++t) {
-            uint32_t block, at;
-            const bool ok = look_up(key0 + t * 16u + col, block, at);
-            seen |= ((uint32_t)__ballot(ok) & 0xffffu) << (16 * t);
-            const char* src = k_base + place(a.k, block, at);
-            for (int n = 0; n < (FP8 ? DP / 64 : DP / 32); ++n) {
-                const uint32_t d = FP8 ? n * 64u + quarter * 16u : n * 32u + quarter * 8u;
-                k_reg[t][n] = u32x4{0, 0, 0, 0};
-                if (d < a.dim) k_reg[t][n] = *reinterpret_cast<const u32x4*>(src + d * (FP8 ? 1u : 2u));
+    const uint32_t tid = threadIdx.x, lane = tid % 64u, wave = __builtin_amdgcn_readfirstlane(tid / 64u), col = lane % 16u, quarter = lane / 16u;
+    const bool is_prefix = blockIdx.x < prefix.groups;
+    const NarrowWalk& w = is_prefix ? prefix : own;
+    const uint32_t group_id = is_prefix ? blockIdx.x : blockIdx.x - prefix.groups;
+    // Workgroups go to the XCDs in turn. Where there are ranges for each, all heads of the same keys go to one: where tokens are
+    // stored whole its L2 then takes whole lines and pages, and the scales' lines once.
+    const uint32_t head_groups = a.cache_heads / HEADS, same_keys = head_groups * w.tiles;
+    const bool by_xcd = w.ranges % 8u == 0;
+    const uint32_t of_range = by_xcd ? group_id / 8u % same_keys : group_id % same_keys;
+    const uint32_t range = by_xcd ? group_id / 8u / same_keys * 8u + group_id % 8u : group_id / same_keys;
+    const uint32_t head = of_range % head_groups * HEADS + wave / kWavesPerHead, tile = of_range / head_groups;
+    const uint32_t key_wave = wave % kWavesPerHead;
+
+    const uint32_t T_block = a.split.T, all = sum_units(w, T_block, 0).all, share = share_of(w, all);
+    if ((uint64_t)range * share >= all) return;
+    uint32_t unit = range * share;
+    const uint32_t end_unit = all - unit < share ? all : unit + share;
+    UnitPlace at_seq = find_unit(w, T_block, unit);
+    // One part of the range after the other: keys [first_key, end_key) of sequence at_seq.seq.
+    for (uint32_t seq = at_seq.seq, start_unit = at_seq.start; unit < end_unit; ++seq) {
+        const uint32_t len = clamp_len(w.lens[seq], w.width, T_block), n_units = (len + kUnit - 1u) / kUnit;
+        const uint32_t stop = start_unit + n_units < end_unit ? start_unit + n_units : end_unit;
+        if (n_units == 0) continue;
+        const uint32_t first_key = (unit - start_unit) * kUnit;
+        const uint32_t end_key = (stop - start_unit) * kUnit < len ? (stop - start_unit) * kUnit : len;
+        unit = stop;
+        start_unit += n_units;
+        const uint32_t n_tile_rows = w.tokens_per_seq * a.group;
+
+        uint32_t token[R], q_head[R];
+        bool owns[R];
+        typename T::Vec8 q[R][kKSteps];
+        for (int r = 0; r < R; ++r) {
+            const uint32_t row = (tile * R + r) * 16u + col;
+            owns[r] = row < n_tile_rows;
+            token[r] = seq * w.tokens_per_seq + (owns[r] ? row / a.group : 0u);
+            q_head[r] = head * a.group + (owns[r] ? row % a.group : 0u);
+            const char* src = a.q + (int64_t)token[r] * a.q_token + (int64_t)q_head[r] * a.q_head;
+            for (int s = 0; s < kKSteps; ++s) {
+                // an e4m3 row is read 16 values at a time, which two steps share
+                const uint32_t d = FP8 ? (s / 2) * 64u + quarter * 16u + (s % 2) * 8u : s * 32u + quarter * 8u;
+                u32x4 x{0, 0, 0, 0};
+                if (owns[r] && d < a.dim) x = *reinterpret_cast<const u32x4*>(src + 2u * d);
+                q[r][s] = as_vec8<T>(x);
             }
-            if constexpr (FP8) k_scale[t] = k_scale_base[scale_place(a.k, block, at)];
         }
-        // The second product's: value j of this quarter is key 16 (j / 4) + 4 quarter + j % 4, in the order in which the first
-        // product leaves its scores; this lane has columns col * kCols ..+kCols-1 of all eight.
-        constexpr int kWords = FP8 ? kCols / 4 : kCols / 2;
-        uint32_t v_reg[8][kWords];
-        float v_scale[8];
-        const uint32_t d0 = col * kCols;
-        for (int t = 0; t < 2; ++t) {
-            uint32_t block = 0, at = 0;
-            bool ok = false;
-            const uint32_t base = key0 + t * 16u + quarter * 4u;
-            // four keys from one look-up: the last of them inside the sequence says nothing of the first, so each
-            // is asked for its own bit of `seen`
-            if (by_four) ok = look_up(base, block, at);
-            for (int j = 0; j < 4; ++j) {
-                if (!by_four) ok = look_up(base + j, block, at);
-                const bool mine = ok && ((seen >> (t * 16u + quarter * 4u + j)) & 1u) != 0;
-                const uint32_t place_at = by_four ? at + j : at;
-                const int64_t where = mine ? place(a.v, block, place_at) : 0;
-                for (int x = 0; x < kWords; ++x) v_reg[4 * t + j][x] = 0;
-                if (mine && d0 < a.dim) {
-                    const char* src = v_base + where + d0 * (FP8 ? 1u : 2u);
-                    if constexpr (kWords == 1) {
-                        v_reg[4 * t + j][0] = *reinterpret_cast<const uint32_t*>(src);
-                    } else if constexpr (kWords == 2) {
-                        const u32x2 x = *reinterpret_cast<const u32x2*>(src);
-                        v_reg[4 * t + j][0] = x[0];
-                        v_reg[4 * t + j][1] = x[1];
-                    } else {
-                        for (int y = 0; y < kWords / 4; ++y) {
-                            const u32x4 x = *reinterpret_cast<const u32x4*>(src + 16 * y);
-                            for (int i = 0; i < 4; ++i) v_reg[4 * t + j][4 * y + i] = x[i];
-                        }
+        f32x4 o[R][kCols];
+        float top[R], sum[R];
+        for (int r = 0; r < R; ++r) {
+            top[r] = kMinusInf;
+            sum[r] = 0.0f;
+            for (int c = 0; c < kCols; ++c) o[r][c] = f32x4{0, 0, 0, 0};
+        }
+
+        const int64_t* table = w.table + (uint64_t)seq * w.width;
+        const char* k_base = a.k.values + (int64_t)head * a.k.head;
+        const char* v_base = a.v.values + (int64_t)head * a.v.head;
+        const float* k_scale_base = FP8 ? a.k.scales + (int64_t)head * a.k.scale_head : nullptr;
+        const float* v_scale_base = FP8 ? a.v.scales + (int64_t)head * a.v.scale_head : nullptr;
+        // A tile of 32 keys. Lane l looks up key l % 32 and, of an e4m3 cache, loads one scale: K's in the lower half, V's in the
+        // upper. A key that is not visible is given the cache's first token: its score is masked and its values are taken for
+        // zeros. Rows are loaded whole by neighbouring lanes, 16 bytes each where they can be: four neighbours then make one
+        // request of 64 bytes, where a lane for each key would make four. K goes through LDS into the first product's order. (24
+        // sequences of 8000 tokens, 8 heads of 128 in e4m3: 98 us; K loaded in the first product's order 104 us.)
+        const uint32_t last_entry = w.width == 0 ? 0u : w.width - 1u;
+        WaveLds& mine = lds.wave[wave];
+        const auto look_up = [&](uint32_t key0) -> int64_t {
+            const uint32_t n = a.split.block32(key0 + lane % 32u);
+            return table[n < last_entry ? n : last_entry];
+        };
+        constexpr int kWords = FP8 ? kCols / 4 : kCols / 2;              // of V per lane and key
+        constexpr int kRowsAtOnce = 64 / kRowPieces, kLoads = 32 / kRowsAtOnce;
+        const uint32_t piece = lane % kRowPieces, piece_row = lane / kRowPieces;
+        const bool piece_exists = piece * (FP8 ? 16u : 8u) < a.dim;
+        const uint32_t d0 = col * kCols < a.dim ? col * kCols : 0u;      // columns that do not exist are computed for nothing
+        constexpr float kLift = kLiftOf<T>;
+        const float lazily = kLazily / a.score_scale;
+        struct Tile32 {
+            u32x4 k[kLoads];
+            uint32_t v[8][kWords];
+            float scale;
+            uint32_t seen;
+        };
+        const auto load_tile = [&](uint32_t key0, int64_t entry) -> Tile32 {
+            Tile32 x;
+            const uint32_t key = key0 + lane % 32u;
+            const bool ok = key < end_key && (uint64_t)entry < a.blocks;
+            x.seen = (uint32_t)__ballot(ok);
+            const uint32_t block = ok ? (uint32_t)entry : 0u, at = ok ? key - a.split.block32(key) * a.split.T : 0u;
+            if constexpr (FP8) x.scale = lane < 32u ? k_scale_base[scale_place(a.k, block, at)] : v_scale_base[scale_place(a.v, block, at)];
+            mine.place[lane % 32u][lane / 32u] = lane < 32u ? place(a.k, block, at) : place(a.v, block, at);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            for (int n = 0; n < kLoads; ++n) {
+                x.k[n] = u32x4{0, 0, 0, 0};
+                const int64_t from = mine.place[n * kRowsAtOnce + piece_row][0];
+                x.k[n] = *reinterpret_cast<const u32x4*>(k_base + from + (piece_exists ? piece * 16u : 0u));
+            }
+            // Value j of this quarter is key 16 (j / 4) + 4 quarter + j % 4, in the order in which the first product leaves its
+            // scores; this lane has columns col * kCols ..+kCols-1 of all eight.
+            for (int j = 0; j < 8; ++j) {
+                const char* src = v_base + mine.place[j / 4 * 16 + quarter * 4 + j % 4][1] + d0 * (FP8 ? 1u : 2u);
+                uint32_t* to = x.v[j];
+                if constexpr (kWords == 1) {
+                    to[0] = *reinterpret_cast<const uint32_t*>(src);
+                } else if constexpr (kWords == 2) {
+                    const u32x2 y = *reinterpret_cast<const u32x2*>(src);
+                    to[0] = y[0];
+                    to[1] = y[1];
+                } else {
+                    for (int n = 0; n < kWords / 4; ++n) {
+                        const u32x4 y = *reinterpret_cast<const u32x4*>(src + 16 * n);
+                        for (int i = 0; i < 4; ++i) to[4 * n + i] = y[i];
                     }
                 }
-                if constexpr (FP8) v_scale[4 * t + j] = mine ? v_scale_base[scale_place(a.v, block, place_at)] : 1.0f;
             }
-        }
-
-        f32x4 s[R][2];
-        for (int r = 0; r < R; ++r)
-            for (int t = 0; t < 2; ++t) s[r][t] = f32x4{0, 0, 0, 0};
-        for (int t = 0; t < 2; ++t)
-            for (int n = 0; n < kKSteps; ++n) {
-                u32x4 x;
-                if constexpr (FP8) {
-                    const uint32_t w0 = k_reg[t][n / 2][2 * (n % 2)], w1 = k_reg[t][n / 2][2 * (n % 2) + 1];
-                    x = u32x4{T::template from_fp8<false>(w0, k_scale[t]), T::template from_fp8<true>(w0, k_scale[t]),
-                              T::template from_fp8<false>(w1, k_scale[t]), T::template from_fp8<true>(w1, k_scale[t])};
-                } else {
-                    x = k_reg[t][n];
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            return x;
+        };
+        const auto compute = [&](Tile32& now) {
+            const uint32_t seen = now.seen;
+            for (int n = 0; n < kLoads; ++n)
+                *reinterpret_cast<u32x4*>(mine.k + (n * kRowsAtOnce + piece_row) * kRowBytes + piece * 16u) = piece_exists ? now.k[n] : u32x4{0, 0, 0, 0};
+            if constexpr (FP8) mine.scale[lane / 32u][lane % 32u] = now.scale;
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            float k_scale[2], v_scale[8];
+            if constexpr (FP8) {
+                for (int t = 0; t < 2; ++t) {
+                    k_scale[t] = mine.scale[0][t * 16 + col];
+                    const f32x4 y = *reinterpret_cast<const f32x4*>(&mine.scale[1][t * 16 + quarter * 4]);
+                    for (int j = 0; j < 4; ++j) v_scale[4 * t + j] = y[j];
                 }
-                for (int r = 0; r < R; ++r) s[r][t] = T::mfma16(as_vec8<T>(x), q[r][n], s[r][t]);
             }
-        if (seen != 0xffffffffu)
+            if (seen != 0xffffffffu)
+                for (int j = 0; j < 8; ++j)
+                    if (((seen >> (j / 4 * 16u + quarter * 4u + j % 4)) & 1u) == 0)
+                        for (int x = 0; x < kWords; ++x) now.v[j][x] = 0u;
+
+            f32x4 s[R][2];
             for (int r = 0; r < R; ++r)
-                for (int t = 0; t < 2; ++t)
-                    for (int i = 0; i < 4; ++i)
-                        if (((seen >> (t * 16u + quarter * 4u + i)) & 1u) == 0) s[r][t][i] = kMinusInf;
-
-        typename T::Vec8 p[R];
-        for (int r = 0; r < R; ++r) {
-            float high = kMinusInf;
-            for (int t = 0; t < 2; ++t)
-                for (int i = 0; i < 4; ++i) high = fmaxf(high, s[r][t][i]);
-            high = max_across_32(max_across_16(high));
-            const float now = fmaxf(top[r], high);
-            const float keep = now == kMinusInf ? 1.0f : __builtin_amdgcn_exp2f((top[r] - now) * a.score_scale);
-            top[r] = now;
-            const float base = now == kMinusInf ? 0.0f : now * a.score_scale - kLift;
-            float e[8], add = 0.0f;
-            for (int t = 0; t < 2; ++t)
-                for (int i = 0; i < 4; ++i) {
-                    e[4 * t + i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][t][i], a.score_scale, -base));
-                    add += e[4 * t + i];
+                for (int t = 0; t < 2; ++t) s[r][t] = f32x4{0, 0, 0, 0};
+            for (int t = 0; t < 2; ++t) {
+                u32x4 raw[kRowPieces / 4];
+                for (int n = 0; n < kRowPieces / 4; ++n)
+                    raw[n] = *reinterpret_cast<const u32x4*>(mine.k + (t * 16 + col) * kRowBytes + (n * 4 + quarter) * 16u);
+                for (int n = 0; n < kKSteps; ++n) {
+                    u32x4 x;
+                    if constexpr (FP8) {
+                        const uint32_t w0 = raw[n / 2][2 * (n % 2)], w1 = raw[n / 2][2 * (n % 2) + 1];
+                        x = u32x4{T::template from_fp8<false>(w0, k_scale[t]), T::template from_fp8<true>(w0, k_scale[t]),
+                                  T::template from_fp8<false>(w1, k_scale[t]), T::template from_fp8<true>(w1, k_scale[t])};
+                    } else {
+                        x = raw[n];
+                    }
+                    for (int r = 0; r < R; ++r) s[r][t] = T::mfma16(as_vec8<T>(x), q[r][n], s[r][t]);
                 }
-            sum[r] = sum[r] * keep + add;
-            for (int c = 0; c < kCols; ++c) o[r][c] *= keep;
-            p[r] = as_vec8<T>(u32x4{T::pack2(e[0], e[1]), T::pack2(e[2], e[3]), T::pack2(e[4], e[5]), T::pack2(e[6], e[7])});
-        }
-        // Columns 2 w and 2 w + 1 of eight keys out of eight dwords.
-        for (int x = 0; x < kCols / 2; ++x) {
-            uint32_t two[8];
-            for (int j = 0; j < 8; ++j) {
-                if constexpr (FP8) two[j] = x % 2 ? T::template from_fp8<true>(v_reg[j][x / 2], v_scale[j]) : T::template from_fp8<false>(v_reg[j][x / 2], v_scale[j]);
-                else two[j] = v_reg[j][x];
             }
-            u32x4 even, odd;
-            for (int i = 0; i < 4; ++i) {
-                even[i] = __builtin_amdgcn_perm(two[2 * i + 1], two[2 * i], 0x05040100u);
-                odd[i] = __builtin_amdgcn_perm(two[2 * i + 1], two[2 * i], 0x07060302u);
-            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            if (seen != 0xffffffffu)
+                for (int r = 0; r < R; ++r)
+                    for (int t = 0; t < 2; ++t)
+                        for (int i = 0; i < 4; ++i)
+                            if (((seen >> (t * 16u + quarter * 4u + i)) & 1u) == 0) s[r][t][i] = kMinusInf;
+
+            typename T::Vec8 p[R];
             for (int r = 0; r < R; ++r) {
-                o[r][2 * x] = T::mfma16(as_vec8<T>(even), p[r], o[r][2 * x]);
-                o[r][2 * x + 1] = T::mfma16(as_vec8<T>(odd), p[r], o[r][2 * x + 1]);
+                float high = kMinusInf;
+                for (int t = 0; t < 2; ++t)
+                    for (int i = 0; i < 4; ++i) high = fmaxf(high, s[r][t][i]);
+                high = max_across_32(max_across_16(high));
+                if (__any(high > top[r] + lazily)) {
+                    const float now = fmaxf(top[r], high);
+                    const float keep = now == kMinusInf ? 1.0f : __builtin_amdgcn_exp2f((top[r] - now) * a.score_scale);
+                    top[r] = now;
+                    sum[r] *= keep;
+                    for (int c = 0; c < kCols; ++c) o[r][c] *= keep;
+                }
+                const float base = top[r] == kMinusInf ? 0.0f : top[r] * a.score_scale - kLift;
+                float e[8], add = 0.0f;
+                for (int t = 0; t < 2; ++t)
+                    for (int i = 0; i < 4; ++i) {
+                        e[4 * t + i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][t][i], a.score_scale, -base));
+                        add += e[4 * t + i];
+                    }
+                sum[r] += add;
+                p[r] = as_vec8<T>(u32x4{T::pack2(e[0], e[1]), T::pack2(e[2], e[3]), T::pack2(e[4], e[5]), T::pack2(e[6], e[7])});
+            }
+            // Columns 2 w and 2 w + 1 of eight keys out of eight dwords.
+            for (int x = 0; x < kCols / 2; ++x) {
+                uint32_t two[8];
+                for (int j = 0; j < 8; ++j) {
+                    if constexpr (FP8) two[j] = x % 2 ? T::template from_fp8<true>(now.v[j][x / 2], v_scale[j]) : T::template from_fp8<false>(now.v[j][x / 2], v_scale[j]);
+                    else two[j] = now.v[j][x];
+                }
+                u32x4 even, odd;
+                for (int i = 0; i < 4; ++i) {
+                    even[i] = __builtin_amdgcn_perm(two[2 * i + 1], two[2 * i], 0x05040100u);
+                    odd[i] = __builtin_amdgcn_perm(two[2 * i + 1], two[2 * i], 0x07060302u);
+                }
+                for (int r = 0; r < R; ++r) {
+                    o[r][2 * x] = T::mfma16(as_vec8<T>(even), p[r], o[r][2 * x]);
+                    o[r][2 * x + 1] = T::mfma16(as_vec8<T>(odd), p[r], o[r][2 * x + 1]);
+                }
+            }
+        };
+        const uint32_t start = first_key + key_wave * 32u;
+        if (start < end_key) {
+            int64_t ahead = look_up(start);      // a tile early; loading the tile itself early was no faster: its registers cost waves
+            for (uint32_t key0 = start; key0 < end_key; key0 += kUnit) {
+                Tile32 now = load_tile(key0, ahead);
+                ahead = look_up(key0 + kUnit);
+                compute(now);
             }
         }
-    }
 
-    // The four waves' sums into wave 0's.
-    for (int r = 0; r < R; ++r) {
-        sum[r] = sum_across_32(sum_across_16(sum[r]));
-        if (quarter == 0) {
-            tops[wave][r * 16 + col] = top[r];
-            sums[wave][r * 16 + col] = sum[r];
-        }
-    }
-    __syncthreads();
-    for (int r = 0; r < R; ++r) {
-        float all = kMinusInf;
-        for (int x = 0; x < 4; ++x) all = fmaxf(all, tops[x][r * 16 + col]);
-        const float keep = top[r] == kMinusInf ? 0.0f : __builtin_amdgcn_exp2f((top[r] - all) * a.score_scale);
-        float total = 0.0f;
-        for (int x = 0; x < 4; ++x) {
-            const float one = tops[x][r * 16 + col];
-            if (one != kMinusInf) total += sums[x][r * 16 + col] * __builtin_amdgcn_exp2f((one - all) * a.score_scale);
-        }
-        for (int c = 0; c < kCols; ++c) o[r][c] *= keep;
-        top[r] = all;
-        sum[r] = total;
-    }
-    for (uint32_t step = 2; step != 0; step >>= 1) {
-        if (wave >= step && wave < 2 * step)
-            for (int r = 0; r < R; ++r)
-                for (int c = 0; c < kCols; ++c)
-                    for (int i = 0; i < 4; ++i) o_lds[wave - step][((r * kCols + c) * 4 + i) * 64 + lane] = o[r][c][i];
-        __syncthreads();
-        if (wave < step)
-            for (int r = 0; r < R; ++r)
-                for (int c = 0; c < kCols; ++c)
-                    for (int i = 0; i < 4; ++i) o[r][c][i] += o_lds[wave][((r * kCols + c) * 4 + i) * 64 + lane];
-        __syncthreads();
-    }
-    if (wave != 0) return;
-    for (int r = 0; r < R; ++r) {
-        if (!owns[r]) continue;
-        const uint64_t row = (uint64_t)token[r] * (a.cache_heads * a.group) + q_head[r];
-        const float high = top[r] == kMinusInf ? kMinusInf : top[r] * a.score_scale - kLift;
-        if (a.part_sum != nullptr) {
-            const uint64_t at = (uint64_t)(w.first_split + split) * a.n_rows * (a.cache_heads * a.group) + row;
-            if (quarter == 0) {
-                a.part_stat[2 * at] = high;
-                a.part_stat[2 * at + 1] = sum[r];
+        for (int r = 0; r < R; ++r) sum[r] = sum_across_32(sum_across_16(sum[r]));
+        if constexpr (HEADS == 1) {      // the four waves' sums into wave 0's
+            for (int r = 0; r < R; ++r) {
+                if (quarter == 0) {
+                    tops[wave][r * 16 + col] = top[r];
+                    sums[wave][r * 16 + col] = sum[r];
+                }
             }
-            if (top[r] == kMinusInf) continue;
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t d = (quarter * 4u + i) * kCols;
-                if (d >= a.dim) continue;
-                for (int c = 0; c < kCols; c += 4)
-                    *reinterpret_cast<f32x4*>(a.part_sum + at * a.dim + d + c) = f32x4{o[r][c][i], o[r][c + 1][i], o[r][c + 2][i], o[r][c + 3][i]};
+            __syncthreads();
+            for (int r = 0; r < R; ++r) {
+                float all = kMinusInf;
+                for (int x = 0; x < 4; ++x) all = fmaxf(all, tops[x][r * 16 + col]);
+                const float keep = top[r] == kMinusInf ? 0.0f : __builtin_amdgcn_exp2f((top[r] - all) * a.score_scale);
+                float total = 0.0f;
+                for (int x = 0; x < 4; ++x) {
+                    const float one = tops[x][r * 16 + col];
+                    if (one != kMinusInf) total += sums[x][r * 16 + col] * __builtin_amdgcn_exp2f((one - all) * a.score_scale);
+                }
+                for (int c = 0; c < kCols; ++c) o[r][c] *= keep;
+                top[r] = all;
+                sum[r] = total;
             }
-        } else {
-            const float inverse = top[r] == kMinusInf ? 0.0f : 1.0f / sum[r];
-            char* dst = a.out + (int64_t)token[r] * a.out_token + (int64_t)q_head[r] * a.out_head;
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t d = (quarter * 4u + i) * kCols;
-                if (d >= a.dim) continue;
-                for (int c = 0; c < kCols; c += 4)
-                    *reinterpret_cast<u32x2*>(dst + 2u * (d + c)) = u32x2{T::pack2(o[r][c][i] * inverse, o[r][c + 1][i] * inverse),
-                                                                        T::pack2(o[r][c + 2][i] * inverse, o[r][c + 3][i] * inverse)};
+            for (uint32_t step = 2; step != 0; step >>= 1) {
+                if (wave >= step && wave < 2 * step)
+                    for (int r = 0; r < R; ++r)
+                        for (int c = 0; c < kCols; ++c)
+                            for (int i = 0; i < 4; ++i) lds.o[wave - step][((r * kCols + c) * 4 + i) * 64 + lane] = o[r][c][i];
+                __syncthreads();
+                if (wave < step)
+                    for (int r = 0; r < R; ++r)
+                        for (int c = 0; c < kCols; ++c)
+                            for (int i = 0; i < 4; ++i) o[r][c][i] += lds.o[wave][((r * kCols + c) * 4 + i) * 64 + lane];
+                __syncthreads();
             }
-            if (a.lse != nullptr && quarter == 0) a.lse[row] = top[r] == kMinusInf ? kMinusInf : (high + __log2f(sum[r])) * kLn2;
         }
+        if (key_wave == 0)
+            for (int r = 0; r < R; ++r) {
+                if (!owns[r]) continue;
+                const uint64_t heads = a.cache_heads * a.group;
+                const uint64_t at = w.n_seqs == 1 ? (uint64_t)range * a.n_rows * heads + token[r] * heads + q_head[r] : ((uint64_t)range + seq) * heads + q_head[r];
+                if (quarter == 0) {
+                    w.to.stat[2 * at] = top[r] == kMinusInf ? kMinusInf : top[r] * a.score_scale - kLift;
+                    w.to.stat[2 * at + 1] = sum[r];
+                }
+                if (top[r] == kMinusInf) continue;
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t d = (quarter * 4u + i) * kCols;
+                    if (d >= a.dim) continue;
+                    for (int c = 0; c < kCols; c += 4)
+                        *reinterpret_cast<f32x4*>(w.to.sum + at * a.dim + d + c) = f32x4{o[r][c][i], o[r][c + 1][i], o[r][c + 2][i], o[r][c + 3][i]};
+                }
+            }
     }
 }
 
 // ---- join -------------------------------------------------------------------------------------
 
-// One wave per query row: the splits' sums, each brought to the common maximum.
-template <typename T>
-__global__ __launch_bounds__(256) void join_splits_kernel(const AttentionArgs a, uint32_t splits, const int64_t* starts, uint32_t n_seqs) {
-    const uint32_t lane = threadIdx.x % 64u, heads = a.cache_heads * a.group;
+struct Join {
+    Partials shared;          // splits that have every row: of a wide launch, or of a narrow one over a prefix
+    uint32_t shared_splits;   // of a wide launch; 0: as many of prefix's ranges as its length takes
+    NarrowWalk prefix, own;   // own.n_seqs == 0: no splits of the rows' own sequences
+    const int64_t* starts;    // of prompts: rows of no sequence have no splits and stay as they are
+    uint32_t n_seqs;
+};
+
+// The splits' sums of a query row, each brought to the common maximum, by WAVES waves of a workgroup: one for many rows, four
+// where rows are few and their splits many.
+template <typename T, int WAVES>
+__global__ __launch_bounds__(256) void join_splits_kernel(const AttentionArgs a, const Join j) {
+    __shared__ f32x4 sums[WAVES][WAVES > 1 ? 64 : 1];
+    __shared__ float totals[WAVES], highs[WAVES];
+    const uint32_t lane = threadIdx.x % 64u, heads = a.cache_heads * a.group, wave = threadIdx.x / 64u % WAVES;
     const uint64_t rows = (uint64_t)a.n_rows * heads;
-    const uint64_t row = (uint64_t)blockIdx.x * 4u + threadIdx.x / 64u;
-    if (row >= rows) return;
-    const uint32_t token = (uint32_t)(row / heads), head = (uint32_t)(row % heads);
-    if (starts != nullptr) {      // rows of no sequence have no splits and stay as they are
+    const uint64_t row = (uint64_t)blockIdx.x * (4u / WAVES) + threadIdx.x / (64u * WAVES);
+    if (row >= rows) return;      // all waves of the row
+    const uint32_t token = __builtin_amdgcn_readfirstlane((uint32_t)(row / heads)), head = (uint32_t)(row % heads);
+    if (j.starts != nullptr) {
         bool inside = false;
-        for (uint32_t b = lane; b < n_seqs; b += 64u) {
-            const int64_t first = starts[b], last = starts[b + 1];
+        for (uint32_t b = lane; b < j.n_seqs; b += 64u) {
+            const int64_t first = j.starts[b], last = j.starts[b + 1];
             inside |= first >= 0 && last <= (int64_t)a.n_rows && (int64_t)token >= first && (int64_t)token < last;
         }
         if (!__any(inside)) return;
     }
-    float high = kMinusInf;
-    for (uint32_t s = lane; s < splits; s += 64u) high = fmaxf(high, a.part_stat[2 * (s * rows + row)]);
-    for (uint32_t o = 32; o != 0; o >>= 1) high = fmaxf(high, __shfl_xor(high, (int)o));
-    float total = 0.0f;
-    f32x4 acc{0, 0, 0, 0};
-    const uint32_t d = lane * 4u;
-    for (uint32_t base = 0; base < splits; base += 64u) {
-        float weight = 0.0f;
-        if (base + lane < splits) {
-            const uint64_t at = (uint64_t)(base + lane) * rows + row;
-            const float top = a.part_stat[2 * at];
-            if (top != kMinusInf) {
-                weight = __builtin_amdgcn_exp2f(top - high);
-                total += weight * a.part_stat[2 * at + 1];
-            }
-        }
-        const uint32_t n = splits - base < 64u ? splits - base : 64u;
-        for (uint32_t s = 0; s < n; ++s) {
-            const float x = __shfl(weight, (int)s);
-            if (x == 0.0f) continue;      // nothing was written there, or it vanishes
-            if (d < a.dim) acc += x * *reinterpret_cast<const f32x4*>(a.part_sum + ((uint64_t)(base + s) * rows + row) * a.dim + d);
+    // The splits there are: first those that have every row, then the parts of this row's own sequence.
+    uint32_t n_shared = j.shared_splits, n_own = 0;
+    if (j.prefix.n_seqs != 0) {
+        const uint32_t all = units_of(j.prefix, a.split.T, 0), share = share_of(j.prefix, all);
+        n_shared = (all + share - 1u) / share;
+    }
+    uint64_t own_at = 0;
+    if (j.own.n_seqs == 1) {
+        const uint32_t all = units_of(j.own, a.split.T, 0), share = share_of(j.own, all);
+        n_own = (all + share - 1u) / share;
+        own_at = head;
+    } else if (j.own.n_seqs != 0) {
+        const UnitSums u = sum_units(j.own, a.split.T, token);
+        const uint32_t mine = units_of(j.own, a.split.T, token), share = share_of(j.own, u.all);
+        if (mine != 0) {
+            const uint32_t first = u.before / share;
+            n_own = (u.before + mine - 1u) / share - first + 1u;
+            own_at = ((uint64_t)first + token) * heads + head;
         }
     }
+    const uint32_t splits = n_shared + n_own;
+    // Place of split s, in rows; of the second kind the next split is `heads` rows further.
+    const auto place_of = [&](uint32_t s) -> uint64_t { return s < n_shared ? s * rows + row : own_at + (uint64_t)(s - n_shared) * heads; };
+    const auto stat_of = [&](uint32_t s) -> const float* { return (s < n_shared ? j.shared.stat : j.own.to.stat) + 2 * place_of(s); };
+
+    // A row of one split takes `lanes` lanes of four values; the wave reads 64 / lanes splits at a time.
+    const uint32_t lanes = a.dim <= 64u ? 16u : a.dim <= 128u ? 32u : 64u, side_by_side = 64u / lanes;
+    const uint32_t d = lane % lanes * 4u, mine = lane / lanes;
+    // One pass: 64 splits' statistics at a time, a running maximum, and four loads of sums in flight that wait for no weight. A
+    // split whose weight is zero may hold anything, or nothing written: it is read and not used.
+    float high = kMinusInf, total = 0.0f;
+    f32x4 acc{0, 0, 0, 0};
+    for (uint32_t base = wave * 64u; base < splits; base += 64u * WAVES) {
+        const uint32_t n = splits - base < 64u ? splits - base : 64u;
+        float top = kMinusInf, sum = 0.0f;
+        if (lane < n) {
+            const float* stat = stat_of(base + lane);
+            top = stat[0];
+            sum = stat[1];
+        }
+        const auto load_sums = [&](uint32_t s, f32x4 (&x)[4]) {
+            for (uint32_t i = 0; i < 4u; ++i) {
+                const uint32_t from = base + s + i * side_by_side + mine;
+                x[i] = f32x4{0, 0, 0, 0};
+                if (from < splits && d < a.dim) x[i] = *reinterpret_cast<const f32x4*>((from < n_shared ? j.shared.sum : j.own.to.sum) + place_of(from) * a.dim + d);
+            }
+        };
+        f32x4 x[4];
+        load_sums(0, x);
+        float most = top;
+        for (uint32_t o = 32; o != 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, (int)o));
+        if (most > high) {
+            const float keep = __builtin_amdgcn_exp2f(high - most);      // 0 at first
+            acc *= keep;
+            total *= keep;
+            high = most;
+        }
+        const float weight = top == kMinusInf ? 0.0f : __builtin_amdgcn_exp2f(top - high);
+        total += weight == 0.0f ? 0.0f : weight * sum;
+        for (uint32_t s = 0; s < n; s += 4u * side_by_side) {
+            if (s != 0) load_sums(s, x);
+            for (uint32_t i = 0; i < 4u; ++i) {
+                const uint32_t from = s + i * side_by_side + mine;
+                float by = __shfl(weight, (int)(from & 63u));              // by all lanes, whether they have such a split or not
+                if (from >= n) by = 0.0f;
+                for (int c = 0; c < 4; ++c) acc[c] += by == 0.0f ? 0.0f : by * x[i][c];
+            }
+        }
+    }
+    for (uint32_t o = lanes; o < 64u; o <<= 1)
+        for (int i = 0; i < 4; ++i) acc[i] += __shfl_xor(acc[i], (int)o);
     for (uint32_t o = 32; o != 0; o >>= 1) total += __shfl_xor(total, (int)o);
+    if constexpr (WAVES > 1) {
+        sums[wave][lane] = acc;
+        if (lane == 0) {
+            totals[wave] = total;
+            highs[wave] = high;
+        }
+        __syncthreads();
+        if (wave != 0) return;
+        for (int x = 1; x < WAVES; ++x) high = fmaxf(high, highs[x]);
+        acc = f32x4{0, 0, 0, 0};
+        total = 0.0f;
+        for (int x = 0; x < WAVES; ++x) {
+            if (highs[x] == kMinusInf) continue;
+            const float keep = __builtin_amdgcn_exp2f(highs[x] - high);
+            acc += keep * sums[x][lane];
+            total += keep * totals[x];
+        }
+    }
     const float inverse = high == kMinusInf ? 0.0f : 1.0f / total;
-    if (d < a.dim) {
+    if (d < a.dim && mine == 0) {
         char* dst = a.out + (int64_t)token * a.out_token + (int64_t)head * a.out_head + 2u * d;
         *reinterpret_cast<u32x2*>(dst) = u32x2{T::pack2(acc[0] * inverse, acc[1] * inverse), T::pack2(acc[2] * inverse, acc[3] * inverse)};
     }
@@ -894,6 +1090,14 @@ __global__ __launch_bounds__(256) void join_splits_kernel(const AttentionArgs a,
 // ---- host -------------------------------------------------------------------------------------
 
 constexpr uint64_t kMostKeys = 1ull << 30;       // of one sequence
+
+// Products of a block's stride, and of a token's inside its block, fit 32 bits.
+bool block_fits(const hfk_cache_plane& p) {
+    const uint64_t e = hfk::type_bytes(p.type), most = 0xffffffffull;
+    const auto fits = [&](uint64_t block, uint64_t token) { return (p.blocks <= 1 || block <= most) && token * (p.block_tokens - 1) <= most; };
+    return fits(e * (uint64_t)p.block_stride, e * (uint64_t)p.token_stride) &&
+           (p.type != HFK_FP8_E4M3 || fits((uint64_t)p.scale_block_stride, (uint64_t)p.scale_token_stride));
+}
 
 int check_attention(const hfk_attention* a) {
     if (a == nullptr) return HFK_ERR_NULL_POINTER;
@@ -909,6 +1113,7 @@ int check_attention(const hfk_attention* a) {
     if (a->q_heads == 0 || a->q_heads % k.heads != 0) return HFK_ERR_BAD_SIZE;
     if (!(a->scale > 0.0f) || !std::isfinite(a->scale)) return HFK_ERR_BAD_SIZE;
     if (a->q_heads > 65535u || a->n_rows > 0x7fffffffull || a->n_rows * a->q_heads > 0x7fffffffull) return HFK_ERR_TOO_LARGE;
+    if (!block_fits(k) || !block_fits(v)) return HFK_ERR_TOO_LARGE;
     if (!hfk::plane_aligned(k, 16) || !hfk::plane_aligned(v, 16) || !hfk::rows_aligned(a->q) || !hfk::rows_aligned(a->out))
         return HFK_ERR_BAD_ALIGNMENT;
     if (a->lse != nullptr && !hfk::multiple_of(a->lse, 4)) return HFK_ERR_BAD_ALIGNMENT;
@@ -917,12 +1122,13 @@ int check_attention(const hfk_attention* a) {
 
 CacheSide side_of(const hfk_cache_plane& p) {
     const int64_t e = hfk::type_bytes(p.type);
-    return {static_cast<const char*>(p.values), p.type == HFK_FP8_E4M3 ? p.scales : nullptr, e * p.block_stride, e * p.token_stride,
-            e * p.head_stride, p.scale_block_stride, p.scale_token_stride, p.scale_head_stride};
+    const bool one = p.blocks <= 1;      // the stride of a single block means nothing
+    return {static_cast<const char*>(p.values), p.type == HFK_FP8_E4M3 ? p.scales : nullptr, e * p.head_stride, p.scale_head_stride,
+            one ? 0u : (uint32_t)(e * p.block_stride), (uint32_t)(e * p.token_stride), one ? 0u : (uint32_t)p.scale_block_stride,
+            (uint32_t)p.scale_token_stride};
 }
 
-// The workspace holds the splits' sums and, behind them, their maxima and sums of weights.
-AttentionArgs fill(const hfk_attention* a, void* workspace, uint64_t splits) {
+AttentionArgs fill(const hfk_attention* a) {
     AttentionArgs x{};
     x.k = side_of(a->k);
     x.v = side_of(a->v);
@@ -940,12 +1146,14 @@ AttentionArgs fill(const hfk_attention* a, void* workspace, uint64_t splits) {
     x.group = a->q_heads / a->k.heads;
     x.dim = a->k.head_dim;
     x.score_scale = a->scale * 1.44269504088896341f;
-    if (splits > 1) {
-        x.part_sum = static_cast<float*>(workspace);
-        x.part_stat = reinterpret_cast<float*>(static_cast<char*>(workspace) +
-                                               hfk::round_up(a->n_rows * a->q_heads * splits * a->k.head_dim * 4, 256));
-    }
     return x;
+}
+
+// `rows` rows of sums and, behind them, of statistics; `at` moves behind both.
+Partials take(char*& at, uint64_t rows, uint32_t dim) {
+    Partials p{reinterpret_cast<float*>(at), reinterpret_cast<float*>(at + hfk::round_up(rows * dim * 4, 256))};
+    at += hfk::partial_bytes(rows, dim);
+    return p;
 }
 
 int check_workspace(void* workspace, uint64_t bytes, uint64_t needed) {
@@ -956,7 +1164,7 @@ int check_workspace(void* workspace, uint64_t bytes, uint64_t needed) {
 }
 
 template <typename T, bool FP8>
-void launch_wide(const AttentionArgs& x, const Walk& w, hipStream_t s) {
+void launch_wide(const AttentionArgs& x, const WideWalk& w, hipStream_t s) {
     switch (hfk::padded_head_dim(x.dim)) {
         case 64: wide_attention_kernel<T, FP8, 64, 64><<<w.groups, kWideThreads, 0, s>>>(x, w); break;
         case 128: wide_attention_kernel<T, FP8, 128, 64><<<w.groups, kWideThreads, 0, s>>>(x, w); break;
@@ -964,27 +1172,36 @@ void launch_wide(const AttentionArgs& x, const Walk& w, hipStream_t s) {
     }
 }
 
-template <typename T, bool FP8, int DP>
-void launch_narrow_rows(const AttentionArgs& x, const Walk& prefix, const Walk& own, uint32_t row_blocks, hipStream_t s) {
+template <typename T, bool FP8, int DP, int HEADS>
+void launch_narrow_rows(const AttentionArgs& x, const NarrowWalk& prefix, const NarrowWalk& own, uint32_t row_blocks, hipStream_t s) {
     const uint32_t grid = prefix.groups + own.groups;
-    if (row_blocks == 1) narrow_attention_kernel<T, FP8, DP, 1><<<grid, 256, 0, s>>>(x, prefix, own);
-    else if (row_blocks == 2) narrow_attention_kernel<T, FP8, DP, 2><<<grid, 256, 0, s>>>(x, prefix, own);
-    else if constexpr (DP != 256) narrow_attention_kernel<T, FP8, DP, 4><<<grid, 256, 0, s>>>(x, prefix, own);
+    if (row_blocks == 1) narrow_attention_kernel<T, FP8, DP, 1, HEADS><<<grid, 256, 0, s>>>(x, prefix, own);
+    else if (row_blocks == 2) narrow_attention_kernel<T, FP8, DP, 2, HEADS><<<grid, 256, 0, s>>>(x, prefix, own);
+    else if constexpr (DP != 256) narrow_attention_kernel<T, FP8, DP, 4, HEADS><<<grid, 256, 0, s>>>(x, prefix, own);
+}
+
+template <typename T, bool FP8, int DP>
+void launch_narrow_heads(const AttentionArgs& x, const NarrowWalk& prefix, const NarrowWalk& own, uint32_t row_blocks, hipStream_t s) {
+    if (hfk::narrow_heads(x.cache_heads) == 4) launch_narrow_rows<T, FP8, DP, 4>(x, prefix, own, row_blocks, s);
+    else launch_narrow_rows<T, FP8, DP, 1>(x, prefix, own, row_blocks, s);
 }
 
 template <typename T, bool FP8>
-void launch_narrow(const AttentionArgs& x, const Walk& prefix, const Walk& own, uint32_t row_blocks, hipStream_t s) {
+void launch_narrow(const AttentionArgs& x, const NarrowWalk& prefix, const NarrowWalk& own, uint32_t row_blocks, hipStream_t s) {
     switch (hfk::padded_head_dim(x.dim)) {
-        case 64: launch_narrow_rows<T, FP8, 64>(x, prefix, own, row_blocks, s); break;
-        case 128: launch_narrow_rows<T, FP8, 128>(x, prefix, own, row_blocks, s); break;
-        default: launch_narrow_rows<T, FP8, 256>(x, prefix, own, row_blocks, s); break;
+        case 64: launch_narrow_heads<T, FP8, 64>(x, prefix, own, row_blocks, s); break;
+        case 128: launch_narrow_heads<T, FP8, 128>(x, prefix, own, row_blocks, s); break;
+        default: launch_narrow_heads<T, FP8, 256>(x, prefix, own, row_blocks, s); break;
     }
 }
 
 template <typename T>
-void launch_join(const AttentionArgs& x, uint32_t splits, const int64_t* starts, uint32_t n_seqs, hipStream_t s) {
+void launch_join(const AttentionArgs& x, const Join& j, hipStream_t s) {
     const uint64_t rows = (uint64_t)x.n_rows * x.cache_heads * x.group;
-    join_splits_kernel<T><<<(uint32_t)((rows + 3) / 4), 256, 0, s>>>(x, splits, starts, n_seqs);
+    const uint64_t most = (uint64_t)j.shared_splits + j.prefix.ranges + j.own.ranges;      // of one row
+    // 64 rows of 250 splits take 37 us with the attention before them by four waves, 56 by one; 1536 rows of 12 splits 8.2 and 7.2 us.
+    if (most > 64 && rows <= 512) join_splits_kernel<T, 4><<<(uint32_t)rows, 256, 0, s>>>(x, j);
+    else join_splits_kernel<T, 1><<<(uint32_t)((rows + 3) / 4), 256, 0, s>>>(x, j);
 }
 
 int finish() {
@@ -1039,8 +1256,8 @@ int hfk_prompt_attention(const hfk_attention* a, const int64_t* block_table, uin
     rc = check_workspace(workspace, workspace_bytes, p.workspace);
     if (rc != HFK_OK) return rc;
     if (p.wide.groups > 0x7fffffffull) return HFK_ERR_TOO_LARGE;
-    const AttentionArgs x = fill(a, workspace, p.wide.splits);
-    Walk w{};
+    const AttentionArgs x = fill(a);
+    WideWalk w{};
     w.table = block_table;
     w.width = x.blocks != 0 ? (uint32_t)table_width : 0;      // a cache without blocks shows nothing
     w.starts = query_starts;
@@ -1050,11 +1267,20 @@ int hfk_prompt_attention(const hfk_attention* a, const int64_t* block_table, uin
     w.tiles = (uint32_t)p.wide.tiles;
     w.splits = p.wide.splits;
     w.groups = (uint32_t)p.wide.groups;
+    char* at = static_cast<char*>(workspace);
+    if (w.splits > 1) w.to = take(at, a->n_rows * a->q_heads * w.splits, x.dim);
     hipStream_t s = static_cast<hipStream_t>(stream);
     by_type(a, [&](auto type, auto fp8) {
         using T = decltype(type);
         launch_wide<T, decltype(fp8)::value>(x, w, s);
-        if (w.splits > 1) launch_join<T>(x, w.splits, query_starts, w.n_seqs, s);
+        if (w.splits > 1) {
+            Join j{};
+            j.shared = w.to;
+            j.shared_splits = w.splits;
+            j.starts = query_starts;
+            j.n_seqs = w.n_seqs;
+            launch_join<T>(x, j, s);
+        }
     });
     return finish();
 }
@@ -1085,40 +1311,60 @@ int hfk_prefix_attention(const hfk_attention* a, const int64_t* prefix_blocks, u
     const hfk::PrefixPlan p = hfk::plan_prefix(a->n_rows, a->q_heads, a->k.heads, a->k.head_dim, prefix, own);
     rc = check_workspace(workspace, workspace_bytes, p.workspace);
     if (rc != HFK_OK) return rc;
-    if (p.wide.groups + p.prefix.groups + p.own.groups > 0x7fffffffull) return HFK_ERR_TOO_LARGE;
-    const AttentionArgs x = fill(a, workspace, p.splits);
-    Walk shared{}, alone{}, none{};
-    shared.table = prefix_blocks;
-    shared.width = x.blocks != 0 ? (uint32_t)n_prefix_blocks : 0;      // a cache without blocks shows nothing
-    shared.lens = prefix_len;
-    shared.n_seqs = 1;
-    shared.tokens_per_seq = (uint32_t)a->n_rows;
-    shared.tiles = (uint32_t)(p.wide_prefix ? p.wide.tiles : p.prefix.row_tiles);
-    shared.splits = p.wide_prefix ? p.wide.splits : p.prefix.splits;
-    shared.chunk = p.prefix.chunk;
-    shared.groups = (uint32_t)(p.wide_prefix ? p.wide.groups : p.prefix.groups);
-    alone.table = block_table;
-    alone.width = x.blocks != 0 ? (uint32_t)table_width : 0;
-    alone.lens = kv_lens;
-    alone.n_seqs = (uint32_t)a->n_rows;
-    alone.tokens_per_seq = 1;
-    alone.tiles = (uint32_t)p.own.row_tiles;
-    alone.splits = p.own.splits;
-    alone.chunk = p.own.chunk;
-    alone.first_split = prefix != 0 ? shared.splits : 0;
-    alone.groups = (uint32_t)p.own.groups;
+    if (p.wide.groups + p.prefix.groups + p.own.groups > 0x7fffffffull || a->n_rows * hfk::ceil_div(own, hfk::narrow_unit(a->k.heads)) > 0x7fffffffull)
+        return HFK_ERR_TOO_LARGE;
+    const AttentionArgs x = fill(a);
+    const bool narrow_prefix = prefix != 0 && !p.wide_prefix;
+    char* at = static_cast<char*>(workspace);
+    Join j{};
+    WideWalk wide{};
+    NarrowWalk none{};
+    if (prefix != 0) j.shared = take(at, a->n_rows * a->q_heads * (p.wide_prefix ? p.wide.splits : p.prefix.ranges), x.dim);
+    if (p.wide_prefix) {
+        wide.table = prefix_blocks;
+        wide.width = x.blocks != 0 ? (uint32_t)n_prefix_blocks : 0;      // a cache without blocks shows nothing
+        wide.lens = prefix_len;
+        wide.n_seqs = 1;
+        wide.tiles = (uint32_t)p.wide.tiles;
+        wide.splits = p.wide.splits;
+        wide.groups = (uint32_t)p.wide.groups;
+        wide.to = j.shared;
+        j.shared_splits = wide.splits;
+    }
+    if (narrow_prefix) {
+        j.prefix.table = prefix_blocks;
+        j.prefix.width = x.blocks != 0 ? (uint32_t)n_prefix_blocks : 0;
+        j.prefix.lens = prefix_len;
+        j.prefix.n_seqs = 1;
+        j.prefix.tokens_per_seq = (uint32_t)a->n_rows;
+        j.prefix.tiles = (uint32_t)p.prefix.row_tiles;
+        j.prefix.unit = hfk::narrow_unit(x.cache_heads);
+        j.prefix.ranges = p.prefix.ranges;
+        j.prefix.groups = (uint32_t)p.prefix.groups;
+        j.prefix.to = j.shared;
+    }
+    j.own.table = block_table;
+    j.own.width = x.blocks != 0 ? (uint32_t)table_width : 0;
+    j.own.lens = kv_lens;
+    j.own.n_seqs = (uint32_t)a->n_rows;
+    j.own.tokens_per_seq = 1;
+    j.own.tiles = (uint32_t)p.own.row_tiles;
+    j.own.unit = hfk::narrow_unit(x.cache_heads);
+    j.own.ranges = p.own.ranges;
+    j.own.groups = (uint32_t)p.own.groups;
+    j.own.to = take(at, hfk::own_splits(p.own, a->n_rows) * a->q_heads, x.dim);
     hipStream_t s = static_cast<hipStream_t>(stream);
     by_type(a, [&](auto type, auto fp8) {
         using T = decltype(type);
         constexpr bool kFp8 = decltype(fp8)::value;
-        if (prefix != 0 && p.wide_prefix) launch_wide<T, kFp8>(x, shared, s);
-        if (prefix != 0 && !p.wide_prefix && p.prefix.row_blocks == p.own.row_blocks) {
-            launch_narrow<T, kFp8>(x, shared, alone, p.own.row_blocks, s);
+        if (p.wide_prefix) launch_wide<T, kFp8>(x, wide, s);
+        if (narrow_prefix && p.prefix.row_blocks == p.own.row_blocks) {
+            launch_narrow<T, kFp8>(x, j.prefix, j.own, p.own.row_blocks, s);
         } else {
-            if (prefix != 0 && !p.wide_prefix) launch_narrow<T, kFp8>(x, shared, none, p.prefix.row_blocks, s);
-            launch_narrow<T, kFp8>(x, none, alone, p.own.row_blocks, s);
+            if (narrow_prefix) launch_narrow<T, kFp8>(x, j.prefix, none, p.prefix.row_blocks, s);
+            launch_narrow<T, kFp8>(x, none, j.own, p.own.row_blocks, s);
         }
-        if (p.splits > 1) launch_join<T>(x, p.splits, nullptr, 0, s);
+        launch_join<T>(x, j, s);
     });
     return finish();
 }

@@ -11,7 +11,11 @@
 namespace hfk {
 
 constexpr uint32_t kWideRows = 256;        // query rows of a wide workgroup
-constexpr uint32_t kMinSplitKeys = 256;    // no split shorter than this: its fixed cost would show
+constexpr uint32_t kMinSplitKeys = 256;    // no split of a wide workgroup's keys shorter than this: its fixed cost would show
+
+// Cache heads of a narrow workgroup's four waves, and the keys they take at a time.
+inline uint32_t narrow_heads(uint32_t cache_heads) { return cache_heads % 4 == 0 ? 4 : 1; }
+inline uint32_t narrow_unit(uint32_t cache_heads) { return 32 * 4 / narrow_heads(cache_heads); }
 
 inline uint64_t ceil_div(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
 inline uint64_t round_up(uint64_t a, uint64_t b) { return ceil_div(a, b) * b; }
@@ -21,10 +25,8 @@ inline uint64_t max64(uint64_t a, uint64_t b) { return a < b ? b : a; }
 // Head sizes are served by the next of these, zero-filled beyond head_dim.
 inline uint32_t padded_head_dim(uint32_t d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 
-// Floats of one row of one split in the workspace: the sum, the largest score (times log2 e), the sum of weights.
-inline uint64_t partial_bytes(uint64_t rows, uint64_t splits, uint32_t head_dim) {
-    return round_up(rows * splits * head_dim * 4, 256) + round_up(rows * splits * 8, 256);
-}
+// Rows of splits in the workspace: a sum each, and behind all of them the largest score (times log2 e) and the sum of weights.
+inline uint64_t partial_bytes(uint64_t rows, uint32_t head_dim) { return round_up(rows * head_dim * 4, 256) + round_up(rows * 8, 256); }
 
 struct WidePlan {
     uint64_t tiles;      // upper bound over the sequences: each one's last tile may be partly filled
@@ -38,7 +40,7 @@ inline WidePlan plan_wide(uint64_t rows, uint64_t n_seqs, uint32_t cache_heads, 
     p.tiles = rows / kWideRows + min64(n_seqs, rows);
     if (n_seqs == 1) p.tiles = ceil_div(rows, kWideRows);
     const uint64_t whole = max64(1, p.tiles * cache_heads);
-    p.splits = (uint32_t)max64(1, min64(ceil_div(wanted_groups, whole), most_keys / kMinSplitKeys));
+    p.splits = (uint32_t)max64(1, min64(wanted_groups / whole, most_keys / kMinSplitKeys));
     p.groups = p.tiles * cache_heads * p.splits;
     return p;
 }
@@ -46,25 +48,27 @@ inline WidePlan plan_wide(uint64_t rows, uint64_t n_seqs, uint32_t cache_heads, 
 struct NarrowPlan {
     uint32_t row_blocks;     // 16 query rows each, per wave: 1, 2 or 4
     uint64_t row_tiles;      // per sequence
-    uint32_t chunk;          // keys of one workgroup, a multiple of 128
-    uint32_t splits;
+    uint32_t ranges;         // shares of all sequences' keys together
     uint64_t groups;
 };
 
-// rows: tokens * group of one sequence.
-inline NarrowPlan plan_narrow(uint64_t rows, uint64_t n_seqs, uint32_t cache_heads, uint32_t head_dim, uint64_t most_keys,
-                              uint64_t wanted_groups) {
+// rows: tokens * group of one sequence; units: the most units of keys that all sequences can have together. As many workgroups
+// as are resident at once, each with an equal share of the keys there are: rounds of more workgroups than that end ragged.
+inline NarrowPlan plan_narrow(uint64_t rows, uint32_t cache_heads, uint32_t head_dim, uint64_t units) {
     NarrowPlan p{};
-    const uint32_t most = padded_head_dim(head_dim) == 256 ? 2 : 4;
+    const uint32_t dim = padded_head_dim(head_dim), most = dim == 256 ? 2 : 4;
     p.row_blocks = rows <= 16 ? 1 : (rows <= 32 || most == 2) ? 2 : 4;
     p.row_tiles = ceil_div(rows, 16ull * p.row_blocks);
-    const uint64_t items = max64(1, p.row_tiles * n_seqs * cache_heads);
-    p.chunk = (uint32_t)round_up(max64(kMinSplitKeys, ceil_div(most_keys * items, wanted_groups)), 128);
-    if (p.chunk > (1u << 30)) p.chunk = 1u << 30;
-    p.splits = (uint32_t)max64(1, ceil_div(most_keys, p.chunk));
-    p.groups = p.row_tiles * n_seqs * cache_heads * p.splits;
+    const uint64_t resident = p.row_blocks * dim <= 256 ? 512 : 256, same_keys = p.row_tiles * (cache_heads / narrow_heads(cache_heads));
+    uint64_t ranges = min64(max64(1, resident / same_keys), max64(1, units));
+    if (ranges > 8) ranges -= ranges % 8;      // the same number for each XCD
+    p.ranges = (uint32_t)ranges;
+    p.groups = ranges * same_keys;
     return p;
 }
+
+// Splits that the parts of n_seqs sequences make (see NarrowWalk).
+inline uint64_t own_splits(const NarrowPlan& p, uint64_t n_seqs) { return n_seqs == 1 ? p.ranges : p.ranges + n_seqs; }
 
 struct PromptPlan {
     WidePlan wide;
@@ -74,16 +78,15 @@ struct PromptPlan {
 inline PromptPlan plan_prompt(uint64_t n_rows, uint32_t q_heads, uint32_t cache_heads, uint32_t head_dim, uint64_t n_seqs,
                               uint64_t most_keys) {
     PromptPlan p{};
-    p.wide = plan_wide(n_rows * (q_heads / cache_heads), n_seqs, cache_heads, most_keys, 512);
-    p.workspace = p.wide.splits > 1 ? partial_bytes(n_rows * q_heads, p.wide.splits, head_dim) : 0;
+    p.wide = plan_wide(n_rows * (q_heads / cache_heads), n_seqs, cache_heads, most_keys, 256);
+    p.workspace = p.wide.splits > 1 ? partial_bytes(n_rows * q_heads * p.wide.splits, head_dim) : 0;
     return p;
 }
 
 struct PrefixPlan {
     bool wide_prefix;        // the prefix goes through the wide kernel (more rows than a narrow workgroup takes)
     WidePlan wide;
-    NarrowPlan prefix, own;  // prefix.splits == 0: no narrow prefix
-    uint32_t splits;         // of prefix and own tokens together
+    NarrowPlan prefix, own;
     uint64_t workspace;
 };
 
@@ -91,20 +94,14 @@ inline PrefixPlan plan_prefix(uint64_t n_rows, uint32_t q_heads, uint32_t cache_
                               uint64_t own_keys) {
     PrefixPlan p{};
     const uint32_t group = q_heads / cache_heads;
-    uint32_t prefix_splits = 0;
     if (prefix_keys != 0) {
         p.wide_prefix = n_rows * group > (padded_head_dim(head_dim) == 256 ? 32 : 64);
-        if (p.wide_prefix) {
-            p.wide = plan_wide(n_rows * group, 1, cache_heads, prefix_keys, 512);
-            prefix_splits = p.wide.splits;
-        } else {
-            p.prefix = plan_narrow(n_rows * group, 1, cache_heads, head_dim, prefix_keys, 1024);
-            prefix_splits = p.prefix.splits;
-        }
+        if (p.wide_prefix) p.wide = plan_wide(n_rows * group, 1, cache_heads, prefix_keys, 256);
+        else p.prefix = plan_narrow(n_rows * group, cache_heads, head_dim, ceil_div(prefix_keys, narrow_unit(cache_heads)));
+        p.workspace += partial_bytes(n_rows * q_heads * (p.wide_prefix ? p.wide.splits : p.prefix.ranges), head_dim);
     }
-    p.own = plan_narrow(group, n_rows, cache_heads, head_dim, own_keys, 8192);
-    p.splits = prefix_splits + p.own.splits;
-    p.workspace = p.splits > 1 ? partial_bytes(n_rows * q_heads, p.splits, head_dim) : 0;
+    p.own = plan_narrow(group, cache_heads, head_dim, n_rows * ceil_div(own_keys, narrow_unit(cache_heads)));
+    p.workspace += partial_bytes(own_splits(p.own, n_rows) * q_heads, head_dim);
     return p;
 }
 

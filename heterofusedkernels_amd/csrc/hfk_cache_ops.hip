@@ -1,8 +1,8 @@
 // Tokens into the paged cache and out of it: hfk_cache_write and hfk_cache_read of include/hfk.h.
 //
-// Both are one pass over the rows: a group of 8 to 64 lanes takes one (token, head) row, 16 bytes of 16-bit values
-// per lane, and keeps it in registers between finding its largest value and writing it (write) or between loading
-// and widening it (read). Keys and values go in one launch, so a decoding step pays one launch for both. What bounds
+// Both are one pass over the rows: a group of lanes takes one (token, head) row, 16 bytes of cached values per lane, and
+// keeps it in registers between finding its largest value and writing it (write) or between loading and widening it
+// (read). Keys and values go in one launch, so a decoding step pays one launch for both. What bounds
 // a long call is HBM traffic, what bounds a short one is the launch.
 #include <hip/hip_runtime.h>
 
@@ -25,7 +25,8 @@ struct Side {
     float* scales;
     int64_t row_token, row_head, block, token, head;      // strides, bytes
     int64_t scale_block, scale_token, scale_head;         // strides, floats
-    uint32_t heads, dim;
+    BlockSplit heads;         // rows of a token
+    uint32_t dim;
     uint32_t lanes;           // per row, a power of two
     uint32_t n_rows;          // tokens * heads
 };
@@ -53,7 +54,7 @@ __device__ Row locate(const Args& a, const Side& s, uint32_t group) {
     Row r{};
     r.lane = threadIdx.x % s.lanes;
     if (row >= s.n_rows) return r;
-    const uint32_t token = (uint32_t)row / s.heads, head = (uint32_t)row % s.heads;
+    const uint32_t token = s.heads.block32((uint32_t)row), head = (uint32_t)row - token * s.heads.T;
     const uint64_t slot = (uint64_t)a.slots[token];      // a negative one is larger than any capacity
     if (slot >= a.capacity) return r;
     const uint64_t block = a.split.block(slot), at = slot - block * a.split.T;
@@ -115,36 +116,51 @@ __device__ void widen(u32x4 v, float (&x)[8]) {
 
 // ---- write -----------------------------------------------------------------------------------
 
-// CHUNKS 16-byte pieces per lane: piece c of lane l is values (c * lanes + l) * 8 ..+7 of the row.
-template <typename T, bool FP8, int CHUNKS>
+// CHUNKS pieces per lane: piece c of lane l is values (c * lanes + l) * PIECE ..+PIECE-1 of the row. PIECE is 8 for 16-bit
+// caches, and 16 for e4m3 where everything is aligned for it: 16 bytes of the cache either way. (8192 tokens of 8 heads of 128,
+// keys and values, from bf16 into e4m3: 12.1 us with 16 values, 4.2 TB/s; 14.5 with 8.)
+template <typename T, bool FP8, int PIECE, int CHUNKS>
 __global__ __launch_bounds__(256) void cache_write_kernel(const Args a) {
+    constexpr int kLoads = PIECE / 8;
     uint32_t group;
     const Side& s = side_of(a, group);
     const Row r = locate(a, s, group);
-    u32x4 v[CHUNKS];
+    u32x4 v[CHUNKS][kLoads];
     for (int c = 0; c < CHUNKS; ++c) {
-        const uint32_t d = (c * s.lanes + r.lane) * 8u;
-        v[c] = u32x4{0, 0, 0, 0};
-        if (r.ok && d < s.dim) v[c] = *reinterpret_cast<const u32x4*>(r.outside + 2 * d);
+        const uint32_t d = (c * s.lanes + r.lane) * PIECE;
+        for (int n = 0; n < kLoads; ++n) {
+            v[c][n] = u32x4{0, 0, 0, 0};
+            if (r.ok && d < s.dim) v[c][n] = *reinterpret_cast<const u32x4*>(r.outside + 2 * d + 16 * n);
+        }
     }
     if constexpr (!FP8) {
         for (int c = 0; c < CHUNKS; ++c) {
-            const uint32_t d = (c * s.lanes + r.lane) * 8u;
-            if (r.ok && d < s.dim) *reinterpret_cast<u32x4*>(r.inside + 2 * d) = v[c];
+            const uint32_t d = (c * s.lanes + r.lane) * PIECE;
+            if (r.ok && d < s.dim) *reinterpret_cast<u32x4*>(r.inside + 2 * d) = v[c][0];
         }
     } else {
-        float x[CHUNKS][8], most = 0.0f;
-        for (int c = 0; c < CHUNKS; ++c) {
-            widen<T>(v[c], x[c]);
-            for (int i = 0; i < 8; ++i) most = fmaxf(most, finite_size(x[c][i]));
-        }
+        float most = 0.0f;
+        for (int c = 0; c < CHUNKS; ++c)
+            for (int n = 0; n < kLoads; ++n) {
+                float x[8];
+                widen<T>(v[c][n], x);
+                for (int i = 0; i < 8; ++i) most = fmaxf(most, finite_size(x[i]));
+            }
         const uint32_t e = scale_exponent(group_max(most, s.lanes));
         const float inverse = __uint_as_float((254u - e) << 23);
         for (int c = 0; c < CHUNKS; ++c) {
-            const uint32_t d = (c * s.lanes + r.lane) * 8u;
-            for (int i = 0; i < 8; ++i) x[c][i] *= inverse;
-            const u32x2 p{four_fp8(x[c][0], x[c][1], x[c][2], x[c][3]), four_fp8(x[c][4], x[c][5], x[c][6], x[c][7])};
-            if (r.ok && d < s.dim) *reinterpret_cast<u32x2*>(r.inside + d) = p;
+            const uint32_t d = (c * s.lanes + r.lane) * PIECE;
+            uint32_t p[PIECE / 4];
+            for (int n = 0; n < kLoads; ++n) {
+                float x[8];
+                widen<T>(v[c][n], x);
+                for (int i = 0; i < 8; ++i) x[i] *= inverse;
+                p[2 * n] = four_fp8(x[0], x[1], x[2], x[3]);
+                p[2 * n + 1] = four_fp8(x[4], x[5], x[6], x[7]);
+            }
+            if (!r.ok || d >= s.dim) continue;
+            if constexpr (PIECE == 16) *reinterpret_cast<u32x4*>(r.inside + d) = u32x4{p[0], p[1], p[2], p[3]};
+            else *reinterpret_cast<u32x2*>(r.inside + d) = u32x2{p[0], p[1]};
         }
         if (r.ok && r.lane == 0) *r.scale = __uint_as_float(e << 23);
     }
@@ -175,35 +191,47 @@ __global__ __launch_bounds__(256) void cache_write_any_kernel(const Args a) {
 
 // ---- read ------------------------------------------------------------------------------------
 
-template <typename T, bool FP8, int CHUNKS>
+// STREAM: the cache is read past the caches, which then keep more of the rows for whoever takes them next.
+template <bool STREAM, typename V>
+__device__ V load_cached(const char* p) {
+    if constexpr (STREAM) return __builtin_nontemporal_load(reinterpret_cast<const V*>(p));
+    else return *reinterpret_cast<const V*>(p);
+}
+
+template <typename T, bool FP8, int PIECE, int CHUNKS, bool STREAM>
 __global__ __launch_bounds__(256) void cache_read_kernel(const Args a) {
+    constexpr int kWords = FP8 ? PIECE / 4 : PIECE / 2;      // of a piece in the cache
     uint32_t group;
     const Side& s = side_of(a, group);
     const Row r = locate(a, s, group);
     if (!r.ok) return;
-    if constexpr (!FP8) {
-        u32x4 v[CHUNKS];
-        for (int c = 0; c < CHUNKS; ++c) {
-            const uint32_t d = (c * s.lanes + r.lane) * 8u;
-            if (d < s.dim) v[c] = *reinterpret_cast<const u32x4*>(r.inside + 2 * d);
+    float scale = 1.0f;
+    if constexpr (FP8) scale = *r.scale;
+    uint32_t v[CHUNKS][kWords];
+    for (int c = 0; c < CHUNKS; ++c) {
+        const uint32_t d = (c * s.lanes + r.lane) * PIECE;
+        if (d >= s.dim) continue;
+        if constexpr (kWords == 4) {
+            const u32x4 x = load_cached<STREAM, u32x4>(r.inside + (FP8 ? d : 2 * d));
+            for (int i = 0; i < 4; ++i) v[c][i] = x[i];
+        } else {
+            const u32x2 x = load_cached<STREAM, u32x2>(r.inside + d);
+            v[c][0] = x[0];
+            v[c][1] = x[1];
         }
-        for (int c = 0; c < CHUNKS; ++c) {
-            const uint32_t d = (c * s.lanes + r.lane) * 8u;
-            if (d < s.dim) *reinterpret_cast<u32x4*>(r.outside + 2 * d) = v[c];
-        }
-    } else {
-        const float scale = *r.scale;
-        u32x2 v[CHUNKS];
-        for (int c = 0; c < CHUNKS; ++c) {
-            const uint32_t d = (c * s.lanes + r.lane) * 8u;
-            if (d < s.dim) v[c] = *reinterpret_cast<const u32x2*>(r.inside + d);
-        }
-        for (int c = 0; c < CHUNKS; ++c) {
-            const uint32_t d = (c * s.lanes + r.lane) * 8u;
-            if (d >= s.dim) continue;
-            const u32x4 w{T::template from_fp8<false>(v[c][0], scale), T::template from_fp8<true>(v[c][0], scale),
-                          T::template from_fp8<false>(v[c][1], scale), T::template from_fp8<true>(v[c][1], scale)};
-            *reinterpret_cast<u32x4*>(r.outside + 2 * d) = w;
+    }
+    for (int c = 0; c < CHUNKS; ++c) {
+        const uint32_t d = (c * s.lanes + r.lane) * PIECE;
+        if (d >= s.dim) continue;
+        if constexpr (!FP8) {
+            *reinterpret_cast<u32x4*>(r.outside + 2 * d) = u32x4{v[c][0], v[c][1], v[c][2], v[c][3]};
+        } else {
+            for (int n = 0; n < PIECE / 8; ++n) {
+                const uint32_t x = v[c][2 * n], y = v[c][2 * n + 1];
+                *reinterpret_cast<u32x4*>(r.outside + 2 * d + 16 * n) =
+                    u32x4{T::template from_fp8<false>(x, scale), T::template from_fp8<true>(x, scale),
+                          T::template from_fp8<false>(y, scale), T::template from_fp8<true>(y, scale)};
+            }
         }
     }
 }
@@ -228,7 +256,7 @@ __global__ __launch_bounds__(256) void cache_read_any_kernel(const Args a) {
 
 // ---- host ------------------------------------------------------------------------------------
 
-int fill_side(Side& s, const hfk_cache_plane& p, const hfk_token_rows& r, uint64_t n, bool vectorised) {
+int fill_side(Side& s, const hfk_cache_plane& p, const hfk_token_rows& r, uint64_t n, uint32_t piece) {
     if (p.head_dim > kMaxHeadDim) return HFK_ERR_TOO_LARGE;
     if (n * p.heads > 0x7fffffffull) return HFK_ERR_TOO_LARGE;
     const int64_t bytes = hfk::type_bytes(p.type);
@@ -243,12 +271,12 @@ int fill_side(Side& s, const hfk_cache_plane& p, const hfk_token_rows& r, uint64
     s.scale_block = p.scale_block_stride;
     s.scale_token = p.scale_token_stride;
     s.scale_head = p.scale_head_stride;
-    s.heads = p.heads;
+    s.heads = BlockSplit::of(p.heads);
     s.dim = p.head_dim;
     s.n_rows = (uint32_t)(n * p.heads);
-    const uint32_t pieces = vectorised ? (p.head_dim + 7u) / 8u : p.head_dim;
+    const uint32_t pieces = (p.head_dim + piece - 1u) / piece, most = piece == 16u ? 16u : 64u;
     s.lanes = 1;
-    while (s.lanes < pieces && s.lanes < 64u) s.lanes *= 2u;
+    while (s.lanes < pieces && s.lanes < most) s.lanes *= 2u;
     return HFK_OK;
 }
 
@@ -259,21 +287,46 @@ int check_side(const hfk_cache_plane& p, const hfk_token_rows& r, uint64_t n) {
     return p.type == HFK_FP8_E4M3 || p.type == r.type ? HFK_OK : HFK_ERR_BAD_TYPE;
 }
 
-bool can_vectorise(const hfk_cache_plane& p, const hfk_token_rows& r) {
-    return p.head_dim % 8u == 0 && hfk::plane_aligned(p, p.type == HFK_FP8_E4M3 ? 8 : 16) && hfk::rows_aligned(r);
+// Values per lane and step: 1 where rows have to be taken value by value.
+uint32_t piece_of(const hfk_cache_plane& p, const hfk_token_rows& r) {
+    if (!hfk::rows_aligned(r)) return 1;
+    if (p.type == HFK_FP8_E4M3 && p.head_dim % 16u == 0 && hfk::plane_aligned(p, 16)) return 16;
+    return p.head_dim % 8u == 0 && hfk::plane_aligned(p, p.type == HFK_FP8_E4M3 ? 8 : 16) ? 8 : 1;
+}
+
+// From this much read and written on, cache_read reads past the caches. Microseconds of a call, and of the call with a
+// kernel behind it that reads the rows (keys and values of 8 heads of 128, e4m3 into bf16; through the caches | past them):
+//   8192 tokens, 51 MB: 12.0, 42.8 | 14.5, 46.1;  16384, 102 MB: 25.5, 63.3 | 22.9, 62.5;  32768, 204 MB: 45.4, 106 | 42.4, 98.
+constexpr uint64_t kStreamBytes = 96ull << 20;
+
+uint64_t moved_bytes(const Args& a, bool fp8) {
+    return (uint64_t)a.side[0].n_rows * a.side[0].dim * (fp8 ? 3 : 4) + (uint64_t)a.side[1].n_rows * a.side[1].dim * (fp8 ? 3 : 4);
+}
+
+template <bool WRITE, typename T, bool FP8, int PIECE, int CHUNKS>
+void launch_pieces(const Args& a, uint32_t grid, hipStream_t s) {
+    if constexpr (WRITE) cache_write_kernel<T, FP8, PIECE, CHUNKS><<<grid, 256, 0, s>>>(a);
+    else if (moved_bytes(a, FP8) < kStreamBytes) cache_read_kernel<T, FP8, PIECE, CHUNKS, false><<<grid, 256, 0, s>>>(a);
+    else cache_read_kernel<T, FP8, PIECE, CHUNKS, true><<<grid, 256, 0, s>>>(a);
 }
 
 template <bool WRITE, typename T, bool FP8>
-void launch_typed(const Args& a, bool vectorised, int chunks, uint32_t grid, hipStream_t s) {
-    if constexpr (WRITE) {
-        if (!vectorised) cache_write_any_kernel<T, FP8><<<grid, 256, 0, s>>>(a);
-        else if (chunks == 1) cache_write_kernel<T, FP8, 1><<<grid, 256, 0, s>>>(a);
-        else cache_write_kernel<T, FP8, 2><<<grid, 256, 0, s>>>(a);
-    } else {
-        if (!vectorised) cache_read_any_kernel<T, FP8><<<grid, 256, 0, s>>>(a);
-        else if (chunks == 1) cache_read_kernel<T, FP8, 1><<<grid, 256, 0, s>>>(a);
-        else cache_read_kernel<T, FP8, 2><<<grid, 256, 0, s>>>(a);
+void launch_typed(const Args& a, uint32_t piece, uint32_t chunks, uint32_t grid, hipStream_t s) {
+    if (piece == 1) {
+        if constexpr (WRITE) cache_write_any_kernel<T, FP8><<<grid, 256, 0, s>>>(a);
+        else cache_read_any_kernel<T, FP8><<<grid, 256, 0, s>>>(a);
+        return;
     }
+    if constexpr (FP8) {
+        if (piece == 16) {      // lanes for 256 values: up to 1024 in four
+            if (chunks == 1) launch_pieces<WRITE, T, FP8, 16, 1>(a, grid, s);
+            else if (chunks == 2) launch_pieces<WRITE, T, FP8, 16, 2>(a, grid, s);
+            else launch_pieces<WRITE, T, FP8, 16, 4>(a, grid, s);
+            return;
+        }
+    }
+    if (chunks == 1) launch_pieces<WRITE, T, FP8, 8, 1>(a, grid, s);
+    else launch_pieces<WRITE, T, FP8, 8, 2>(a, grid, s);
 }
 
 template <bool WRITE>
@@ -291,21 +344,26 @@ int move_tokens(const hfk_cache_plane* kp, const hfk_token_rows* k, const hfk_ca
     if (n > 0x7fffffffull) return HFK_ERR_TOO_LARGE;
     if (n == 0 || kp->blocks == 0) return HFK_OK;
     if (slots == nullptr) return HFK_ERR_NULL_POINTER;
-    const bool vectorised = can_vectorise(*kp, *k) && (vp == nullptr || can_vectorise(*vp, *v));
+    uint32_t piece = piece_of(*kp, *k);
+    if (vp != nullptr) {
+        const uint32_t other = piece_of(*vp, *v);
+        if (other < piece) piece = other;
+    }
     Args a{};
     a.slots = slots;
     a.capacity = kp->blocks * kp->block_tokens;
     a.split = BlockSplit::of(kp->block_tokens);
-    rc = fill_side(a.side[0], *kp, *k, n, vectorised);
-    if (rc == HFK_OK && vp != nullptr) rc = fill_side(a.side[1], *vp, *v, n, vectorised);
+    rc = fill_side(a.side[0], *kp, *k, n, piece);
+    if (rc == HFK_OK && vp != nullptr) rc = fill_side(a.side[1], *vp, *v, n, piece);
     if (rc != HFK_OK) return rc;
     uint64_t groups[2] = {0, 0};
-    int chunks = 1;
+    uint32_t chunks = 1;
     for (int i = 0; i < (vp != nullptr ? 2 : 1); ++i) {
         const Side& s = a.side[i];
         const uint32_t per_group = 256u / s.lanes;
         groups[i] = ((uint64_t)s.n_rows + per_group - 1) / per_group;
-        if (s.lanes * 8u < s.dim) chunks = 2;
+        const uint32_t its = (s.dim + s.lanes * piece - 1u) / (s.lanes * piece);
+        if (its > chunks) chunks = its;
     }
     if (groups[0] + groups[1] > 0x7fffffffull) return HFK_ERR_TOO_LARGE;
     a.first_groups = (uint32_t)groups[0];
@@ -313,11 +371,11 @@ int move_tokens(const hfk_cache_plane* kp, const hfk_token_rows* k, const hfk_ca
     hipStream_t s = static_cast<hipStream_t>(stream);
     const bool fp8 = kp->type == HFK_FP8_E4M3;
     if (k->type == HFK_BF16) {
-        if (fp8) launch_typed<WRITE, hfk::Bf16, true>(a, vectorised, chunks, grid, s);
-        else launch_typed<WRITE, hfk::Bf16, false>(a, vectorised, chunks, grid, s);
+        if (fp8) launch_typed<WRITE, hfk::Bf16, true>(a, piece, chunks, grid, s);
+        else launch_typed<WRITE, hfk::Bf16, false>(a, piece, chunks, grid, s);
     } else {
-        if (fp8) launch_typed<WRITE, hfk::Fp16, true>(a, vectorised, chunks, grid, s);
-        else launch_typed<WRITE, hfk::Fp16, false>(a, vectorised, chunks, grid, s);
+        if (fp8) launch_typed<WRITE, hfk::Fp16, true>(a, piece, chunks, grid, s);
+        else launch_typed<WRITE, hfk::Fp16, false>(a, piece, chunks, grid, s);
     }
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? HFK_OK : (int)e;

@@ -131,15 +131,17 @@ __device__ int64_t scale_place(const CacheSide& s, uint32_t block, uint32_t at) 
 // Which rows a workgroup has: tile `tile` of all the sequences' tiles of ROWS rows.
 struct Tile {
     uint32_t seq, first_token, tokens, first_row;
+    int64_t len;              // of the sequence's keys, as given: loaded beside the starts, not behind them
     bool found;
 };
 
 template <uint32_t ROWS>
 __device__ Tile find_tile(const AttentionArgs& a, const WideWalk& w, uint32_t tile) {
-    Tile t{0, 0, 0, 0, false};
+    Tile t{0, 0, 0, 0, 0, false};
     if (w.starts == nullptr) {
         t.tokens = a.n_rows;
         t.first_row = tile * ROWS;
+        t.len = w.lens[0];
         t.found = t.first_row < t.tokens * a.group;
         return t;
     }
@@ -147,10 +149,11 @@ __device__ Tile find_tile(const AttentionArgs& a, const WideWalk& w, uint32_t ti
     uint32_t before = 0;
     for (uint32_t base = 0; base < w.n_seqs; base += 64u) {       // 64 sequences at a time, by every wave alike
         const uint32_t b = base + lane;
-        int64_t first = 0, last = 0;
+        int64_t first = 0, last = 0, len = 0;
         if (b < w.n_seqs) {
             first = w.starts[b];
             last = w.starts[b + 1];
+            len = w.lens[b];
         }
         const bool sound = first >= 0 && last > first && last <= (int64_t)a.n_rows;
         const uint32_t tokens = sound ? (uint32_t)(last - first) : 0u;
@@ -167,6 +170,8 @@ __device__ Tile find_tile(const AttentionArgs& a, const WideWalk& w, uint32_t ti
             t.first_token = __builtin_amdgcn_readlane((uint32_t)first, at);
             t.tokens = __builtin_amdgcn_readlane(tokens, at);
             t.first_row = (tile - before - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(mine, at))) * ROWS;
+            t.len = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)((uint64_t)len >> 32), at) << 32 |
+                              (uint32_t)__builtin_amdgcn_readlane((uint32_t)len, at));
             t.found = true;
             return t;
         }
@@ -234,7 +239,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(const A
     if (!t.found) return;
 
     const uint32_t n_tile_rows = t.tokens * a.group;
-    const uint32_t len = clamp_len(w.lens[t.seq], w.width, a.split.T);
+    const uint32_t len = clamp_len(t.len, w.width, a.split.T);
     // Keys that a token sees: all, or (causal) so many that the last token sees all.
     const auto seen_by = [&](uint32_t token) -> int32_t {
         if (!w.causal) return (int32_t)len;
@@ -491,7 +496,26 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(const A
     // then a barrier swaps them. The second half starts one barrier late. A tile is put into its stage by both halves'
     // threads one turn before the first half reads it; the stage, one of three, was last read two turns earlier.
     if (tid == 0) not_finite = 0u;
-    if (n_tiles != 0) {
+    if (n_tiles == 1) {      // nothing to overlap with, and nothing to load ahead: a short prompt's latency
+        if (wave == 0) put_keys(0, load_entry(0));
+        __syncthreads();
+        const uint64_t seen = as_scalar(keys[0].seen);
+        read_k_places(0);
+        read_v_places(0);
+        load_k(k_reg);
+        load_v();
+        store_k(0, k_reg);
+        store_v(0, seen);
+        __syncthreads();
+        if (any_row) {
+            first_product(0);
+            hide(0, seen);
+            raise();
+            read_ahead(0);
+            weigh();
+            second_product(0);
+        }
+    } else if (n_tiles != 0) {
         const bool late = wave >= kWaves / 2;
         if (wave == 0) {      // tiles behind the last show nothing
             int64_t first[6];
@@ -647,28 +671,46 @@ __device__ uint32_t share_of(const NarrowWalk& w, uint32_t all) {
     return n == 0 ? 1u : n;
 }
 
-// The sequence that unit `unit` is in, and its first unit. There is one: unit < all.
+// The sequence that unit `unit` is in, its first unit and its length. There is one: unit < all.
 struct UnitPlace {
-    uint32_t seq, start;
+    uint32_t seq, start, len;
 };
-__device__ UnitPlace find_unit(const NarrowWalk& w, uint32_t T, uint32_t unit) {
+// `lens` of 64 sequences from `base` on, a lane each; `before`: the units of those before them.
+__device__ bool find_unit_in(const NarrowWalk& w, uint32_t len, uint32_t base, uint32_t unit, uint32_t& before, UnitPlace& found) {
+    const uint32_t lane = threadIdx.x % 64u, mine = (len + w.unit - 1u) / w.unit;
+    uint32_t upto = mine;
+    for (uint32_t o = 1; o < 64u; o <<= 1) {
+        const uint32_t other = __shfl_up(upto, o);
+        if (lane >= o) upto += other;
+    }
+    const uint64_t past = __ballot(before + upto > unit);
+    if (past != 0) {
+        const int at = __builtin_ctzll(past);
+        found = {base + at, before + (uint32_t)__builtin_amdgcn_readlane(upto, at) - (uint32_t)__builtin_amdgcn_readlane(mine, at),
+                 (uint32_t)__builtin_amdgcn_readlane(len, at)};
+        return true;
+    }
+    before += __builtin_amdgcn_readlane(upto, 63);
+    return false;
+}
+
+// The units of range `range`: [first, end), and where the first lies. false: there are none.
+__device__ bool find_range(const NarrowWalk& w, uint32_t T, uint32_t range, uint32_t& first, uint32_t& end, UnitPlace& found) {
     const uint32_t lane = threadIdx.x % 64u;
+    uint32_t len = lane < w.n_seqs ? clamp_len(w.lens[lane], w.width, T) : 0u, all = (len + w.unit - 1u) / w.unit;
+    for (uint32_t b = lane + 64u; b < w.n_seqs; b += 64u) all += units_of(w, T, b);
+    for (uint32_t o = 32; o != 0; o >>= 1) all += __shfl_xor(all, (int)o);
+    all = __builtin_amdgcn_readfirstlane(all);
+    const uint32_t share = share_of(w, all);
+    if ((uint64_t)range * share >= all) return false;
+    first = range * share;
+    end = all - first < share ? all : first + share;
     uint32_t before = 0;
     for (uint32_t base = 0; base < w.n_seqs; base += 64u) {
-        const uint32_t b = base + lane, mine = b < w.n_seqs ? units_of(w, T, b) : 0u;
-        uint32_t upto = mine;
-        for (uint32_t o = 1; o < 64u; o <<= 1) {
-            const uint32_t other = __shfl_up(upto, o);
-            if (lane >= o) upto += other;
-        }
-        const uint64_t past = __ballot(before + upto > unit);
-        if (past != 0) {
-            const int at = __builtin_ctzll(past);
-            return {base + at, before + (uint32_t)__builtin_amdgcn_readlane(upto, at) - (uint32_t)__builtin_amdgcn_readlane(mine, at)};
-        }
-        before += __builtin_amdgcn_readlane(upto, 63);
+        if (base != 0) len = base + lane < w.n_seqs ? clamp_len(w.lens[base + lane], w.width, T) : 0u;
+        if (find_unit_in(w, len, base, first, before, found)) return true;
     }
-    return {w.n_seqs, before};
+    return false;
 }
 
 // HEADS == 4: a wave for each of four neighbouring cache heads, all at the same keys. HEADS == 1: four waves at one head, whose
@@ -704,14 +746,13 @@ __global__ __launch_bounds__(256, R * DP <= 256 ? 2 : 1) void narrow_attention_k
     const uint32_t head = of_range % head_groups * HEADS + wave / kWavesPerHead, tile = of_range / head_groups;
     const uint32_t key_wave = wave % kWavesPerHead;
 
-    const uint32_t T_block = a.split.T, all = sum_units(w, T_block, 0).all, share = share_of(w, all);
-    if ((uint64_t)range * share >= all) return;
-    uint32_t unit = range * share;
-    const uint32_t end_unit = all - unit < share ? all : unit + share;
-    UnitPlace at_seq = find_unit(w, T_block, unit);
-    // One part of the range after the other: keys [first_key, end_key) of sequence at_seq.seq.
+    const uint32_t T_block = a.split.T;
+    uint32_t unit = 0, end_unit = 0;
+    UnitPlace at_seq{};
+    if (!find_range(w, T_block, range, unit, end_unit, at_seq)) return;
+    // One part of the range after the other: keys [first_key, end_key) of sequence `seq`.
     for (uint32_t seq = at_seq.seq, start_unit = at_seq.start; unit < end_unit; ++seq) {
-        const uint32_t len = clamp_len(w.lens[seq], w.width, T_block), n_units = (len + kUnit - 1u) / kUnit;
+        const uint32_t len = seq == at_seq.seq ? at_seq.len : clamp_len(w.lens[seq], w.width, T_block), n_units = (len + w.unit - 1u) / w.unit;
         const uint32_t stop = start_unit + n_units < end_unit ? start_unit + n_units : end_unit;
         if (n_units == 0) continue;
         const uint32_t first_key = (unit - start_unit) * kUnit;

@@ -583,6 +583,8 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(const A
     }
 
     const float total = sum_across_32(sum);
+    // All scores NaN: no maximum was found, but something was seen, and the sums say what.
+    if (top == kMinusInf && total != total) top = 0.0f;
     const uint64_t heads = a.cache_heads * a.group;
     if (owns) {
         const uint64_t place = (uint64_t)token * heads + q_head;
@@ -751,7 +753,7 @@ __global__ __launch_bounds__(256, R * DP <= 256 ? 2 : 1) void narrow_attention_k
     UnitPlace at_seq{};
     if (!find_range(w, T_block, range, unit, end_unit, at_seq)) return;
     // One part of the range after the other: keys [first_key, end_key) of sequence `seq`.
-    for (uint32_t seq = at_seq.seq, start_unit = at_seq.start; unit < end_unit; ++seq) {
+    for (uint32_t seq = at_seq.seq, start_unit = at_seq.start; unit < end_unit && seq < w.n_seqs; ++seq) {
         const uint32_t len = seq == at_seq.seq ? at_seq.len : clamp_len(w.lens[seq], w.width, T_block), n_units = (len + w.unit - 1u) / w.unit;
         const uint32_t stop = start_unit + n_units < end_unit ? start_unit + n_units : end_unit;
         if (n_units == 0) continue;
@@ -946,7 +948,11 @@ __global__ __launch_bounds__(256, R * DP <= 256 ? 2 : 1) void narrow_attention_k
             }
         }
 
-        for (int r = 0; r < R; ++r) sum[r] = sum_across_32(sum_across_16(sum[r]));
+        for (int r = 0; r < R; ++r) {
+            sum[r] = sum_across_32(sum_across_16(sum[r]));
+            // All scores NaN: no maximum was found, but something was seen, and the sums say what.
+            if (top[r] == kMinusInf && sum[r] != sum[r]) top[r] = 0.0f;
+        }
         if constexpr (HEADS == 1) {      // the four waves' sums into wave 0's
             for (int r = 0; r < R; ++r) {
                 if (quarter == 0) {
@@ -1279,7 +1285,7 @@ int hfk_prompt_attention_workspace(const hfk_attention* a, uint64_t n_seqs, uint
     int rc = check_attention(a);
     if (rc == HFK_OK) rc = most_keys(table_width, a->k.block_tokens, keys);
     if (rc != HFK_OK) return rc;
-    *bytes = hfk::plan_prompt(a->n_rows, a->q_heads, a->k.heads, a->k.head_dim, n_seqs, keys).workspace;
+    *bytes = n_seqs == 0 || a->n_rows == 0 ? 0 : hfk::plan_prompt(a->n_rows, a->q_heads, a->k.heads, a->k.head_dim, n_seqs, keys).workspace;
     return HFK_OK;
 }
 
@@ -1333,7 +1339,7 @@ int hfk_prefix_attention_workspace(const hfk_attention* a, uint64_t n_prefix_blo
     if (rc == HFK_OK) rc = most_keys(table_width, a->k.block_tokens, own);
     if (rc == HFK_OK) rc = most_keys(n_prefix_blocks, a->k.block_tokens, prefix);
     if (rc != HFK_OK) return rc;
-    *bytes = hfk::plan_prefix(a->n_rows, a->q_heads, a->k.heads, a->k.head_dim, prefix, own).workspace;
+    *bytes = a->n_rows == 0 ? 0 : hfk::plan_prefix(a->n_rows, a->q_heads, a->k.heads, a->k.head_dim, prefix, own).workspace;
     return HFK_OK;
 }
 

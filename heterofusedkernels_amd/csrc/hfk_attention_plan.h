@@ -1,5 +1,7 @@
 // Launch planning of the attention entry points: plain C++, no device code, so that it can be checked without a GPU.
 //
+// The plans are made for at least one row and one sequence.
+//
 // Two kernels do the work. The wide one gives a workgroup a tile of query rows (a row is a token and a query head
 // of one cache head's group) and walks keys and values through LDS, shared by its waves: many rows per key, bound by
 // the matrix units. The narrow one gives every wave of a workgroup its own keys straight from memory for up to 64

@@ -79,3 +79,31 @@ def swap_flags(dst_planes, src_planes, beside_compute=False):
     if not side(src_planes, "source"):
         flags |= SWAP_SRC_HOST
     return flags
+
+
+def fp8_block_bytes(block_tokens, heads, head_dim):
+    """Bytes of one block of an e4m3 cache plane that carries its scales: the values
+    [block_tokens, heads, head_dim], then a float32 scale per token and head."""
+    if head_dim % 16 != 0:
+        raise ValueError("head_dim must be a multiple of 16, got %d" % head_dim)
+    return block_tokens * heads * (head_dim + 4)
+
+
+def fp8_cache_views(plane, block_tokens, heads, head_dim):
+    """(values, scales) of a plane of such blocks, ``plane`` being a contiguous uint8 tensor
+    ``[blocks, fp8_block_bytes(...)]``: float8_e4m3fn ``[blocks, block_tokens, heads, head_dim]`` and float32
+    ``[blocks, block_tokens, heads]`` views of its memory, as cache_write, cache_read and the attention ops take them.
+    swap_blocks, gather_blocks and their like move such a plane's blocks with their scales in one go."""
+    import torch
+
+    size = fp8_block_bytes(block_tokens, heads, head_dim)
+    if plane.dtype != torch.uint8 or plane.dim() != 2 or plane.shape[1] != size or not plane.is_contiguous():
+        raise ValueError("plane must be a contiguous uint8 tensor [blocks, %d]" % size)
+    blocks, values = plane.shape[0], block_tokens * heads * head_dim
+    if plane.data_ptr() % 16 != 0 or size % 16 != 0:
+        raise ValueError("blocks must begin at multiples of 16 bytes: block_tokens * heads must be a multiple of 4")
+    v = plane.view(torch.float8_e4m3fn).as_strided((blocks, block_tokens, heads, head_dim),
+                                                   (size, heads * head_dim, head_dim, 1), plane.storage_offset())
+    s = plane.view(torch.float32).as_strided((blocks, block_tokens, heads), (size // 4, heads, 1),
+                                             (plane.storage_offset() + values) // 4)
+    return v, s

@@ -121,6 +121,21 @@ __device__ typename T::Vec8 as_vec8(V v) {
     return __builtin_bit_cast(typename T::Vec8, v);
 }
 
+// Eight weights as an operand, and what rounding them to 16 bits took away as another: with a second product of those the
+// weights are as good as 32 bits. That one has sums of its own, which count where the first one's are numbers: with V
+// infinite it would give NaN where the first gives infinity.
+template <typename T>
+__device__ typename T::Vec8 pack8(const float (&e)[8]) {
+    return as_vec8<T>(u32x4{T::pack2(e[0], e[1]), T::pack2(e[2], e[3]), T::pack2(e[4], e[5]), T::pack2(e[6], e[7])});
+}
+template <typename T>
+__device__ typename T::Vec8 rest8(const float (&e)[8], typename T::Vec8 p) {
+    float rest[8];
+    for (int i = 0; i < 8; ++i) rest[i] = e[i] - (float)p[i];
+    return pack8<T>(rest);
+}
+__device__ float with_rest(float sum, float rest) { return fabsf(sum) <= 3.402823466e38f ? sum + rest : sum; }
+
 __device__ int64_t place(const CacheSide& s, uint32_t block, uint32_t at) { return (int64_t)((uint64_t)block * s.block + at * s.token); }
 __device__ int64_t scale_place(const CacheSide& s, uint32_t block, uint32_t at) {
     return (int64_t)((uint64_t)block * s.scale_block + at * s.scale_token);
@@ -455,7 +470,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(const A
                 for (int i = 0; i < 16; ++i) o[b][i] *= keep;
         }
     };
-    const auto weigh = [&]() {
+    const auto weigh = [&] {
         const float base = top == kMinusInf ? 0.0f : top * a.score_scale - kLift;
         float add = 0.0f;
         for (int b = 0; b < KEYS / 32; ++b)
@@ -465,7 +480,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(const A
                     e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x.s[b][8 * h + i], a.score_scale, -base));
                     add += e[i];
                 }
-                y.p[2 * b + h] = as_vec8<T>(u32x4{T::pack2(e[0], e[1]), T::pack2(e[2], e[3]), T::pack2(e[4], e[5]), T::pack2(e[6], e[7])});
+                y.p[2 * b + h] = pack8<T>(e);
             }
         sum += add;
     };
@@ -722,6 +737,9 @@ __global__ __launch_bounds__(256, R * DP <= 256 ? 2 : 1) void narrow_attention_k
     constexpr int kKSteps = DP / 32;        // matrix instructions of the first product
     constexpr int kCols = DP / 16;          // values of V per lane and key
     constexpr uint32_t kRegs = R * kCols * 4, kWavesPerHead = 4 / HEADS, kUnit = kWavesPerHead * 32;
+    // The weights' rest (see rest8) where the kernel waits for memory and has registers to spare: 83.2 us without and with it
+    // for the decoding step of 24 sequences, 11.5 and 11.9 for one sequence, whose errors then are the output's own rounding.
+    constexpr bool kRest = R * DP <= 128;
     constexpr int kRowPieces = FP8 ? DP / 16 : DP / 8;                   // 16-byte pieces of a cached row
     constexpr uint32_t kRowBytes = kRowPieces * 16 + 16;                 // of K in LDS: 16 rows' pieces of one column, no bank twice
     struct WaveLds {                                                     // a wave's own: no barrier, LDS serves a wave in order
@@ -780,12 +798,15 @@ __global__ __launch_bounds__(256, R * DP <= 256 ? 2 : 1) void narrow_attention_k
                 q[r][s] = as_vec8<T>(x);
             }
         }
-        f32x4 o[R][kCols];
+        f32x4 o[R][kCols], o_rest[kRest ? R : 1][kRest ? kCols : 1];
         float top[R], sum[R];
         for (int r = 0; r < R; ++r) {
             top[r] = kMinusInf;
             sum[r] = 0.0f;
-            for (int c = 0; c < kCols; ++c) o[r][c] = f32x4{0, 0, 0, 0};
+            for (int c = 0; c < kCols; ++c) {
+                o[r][c] = f32x4{0, 0, 0, 0};
+                if constexpr (kRest) o_rest[r][c] = f32x4{0, 0, 0, 0};
+            }
         }
 
         const int64_t* table = w.table + (uint64_t)seq * w.width;
@@ -897,7 +918,7 @@ __global__ __launch_bounds__(256, R * DP <= 256 ? 2 : 1) void narrow_attention_k
                         for (int i = 0; i < 4; ++i)
                             if (((seen >> (t * 16u + quarter * 4u + i)) & 1u) == 0) s[r][t][i] = kMinusInf;
 
-            typename T::Vec8 p[R];
+            typename T::Vec8 p[R], rest[kRest ? R : 1];
             for (int r = 0; r < R; ++r) {
                 float high = kMinusInf;
                 for (int t = 0; t < 2; ++t)
@@ -908,7 +929,10 @@ __global__ __launch_bounds__(256, R * DP <= 256 ? 2 : 1) void narrow_attention_k
                     const float keep = now == kMinusInf ? 1.0f : __builtin_amdgcn_exp2f((top[r] - now) * a.score_scale);
                     top[r] = now;
                     sum[r] *= keep;
-                    for (int c = 0; c < kCols; ++c) o[r][c] *= keep;
+                    for (int c = 0; c < kCols; ++c) {
+                        o[r][c] *= keep;
+                        if constexpr (kRest) o_rest[r][c] *= keep;
+                    }
                 }
                 const float base = top[r] == kMinusInf ? 0.0f : top[r] * a.score_scale - kLift;
                 float e[8], add = 0.0f;
@@ -918,7 +942,8 @@ __global__ __launch_bounds__(256, R * DP <= 256 ? 2 : 1) void narrow_attention_k
                         add += e[4 * t + i];
                     }
                 sum[r] += add;
-                p[r] = as_vec8<T>(u32x4{T::pack2(e[0], e[1]), T::pack2(e[2], e[3]), T::pack2(e[4], e[5]), T::pack2(e[6], e[7])});
+                p[r] = pack8<T>(e);
+                if constexpr (kRest) rest[r] = rest8<T>(e, p[r]);
             }
             // Columns 2 w and 2 w + 1 of eight keys out of eight dwords.
             for (int x = 0; x < kCols / 2; ++x) {
@@ -935,6 +960,10 @@ __global__ __launch_bounds__(256, R * DP <= 256 ? 2 : 1) void narrow_attention_k
                 for (int r = 0; r < R; ++r) {
                     o[r][2 * x] = T::mfma16(as_vec8<T>(even), p[r], o[r][2 * x]);
                     o[r][2 * x + 1] = T::mfma16(as_vec8<T>(odd), p[r], o[r][2 * x + 1]);
+                    if constexpr (kRest) {
+                        o_rest[r][2 * x] = T::mfma16(as_vec8<T>(even), rest[r], o_rest[r][2 * x]);
+                        o_rest[r][2 * x + 1] = T::mfma16(as_vec8<T>(odd), rest[r], o_rest[r][2 * x + 1]);
+                    }
                 }
             }
         };
@@ -952,6 +981,9 @@ __global__ __launch_bounds__(256, R * DP <= 256 ? 2 : 1) void narrow_attention_k
             sum[r] = sum_across_32(sum_across_16(sum[r]));
             // All scores NaN: no maximum was found, but something was seen, and the sums say what.
             if (top[r] == kMinusInf && sum[r] != sum[r]) top[r] = 0.0f;
+            if constexpr (kRest)
+                for (int c = 0; c < kCols; ++c)
+                    for (int i = 0; i < 4; ++i) o[r][c][i] = with_rest(o[r][c][i], o_rest[r][c][i]);
         }
         if constexpr (HEADS == 1) {      // the four waves' sums into wave 0's
             for (int r = 0; r < R; ++r) {

@@ -527,8 +527,10 @@ typedef struct hfk_attention {
  *   workspace     device memory of hfk_prompt_attention_workspace() bytes, 256-byte aligned (NULL if that is 0),
  *                 written and read by this call alone until the stream has passed it
  * Types: q and out HFK_BF16 or HFK_FP16; the cache of the same type or HFK_FP8_E4M3. Scores, statistics
- * and sums are held in 32 bits; the weights are rounded to q's type for the second product.
- * head_dim: a multiple of 16 up to 256. All pointers and strides multiples of 16 bytes.
+ * and sums are held in 32 bits. The second product takes the weights in q's type; where a launch waits for
+ * memory (few rows per cache head, head_dim up to 128) it takes their rounding error too, as a second operand.
+ * head_dim: a multiple of 16 up to 256. All pointers and strides multiples of 16 bytes. A block spans less than
+ * 4 GiB and a sequence or the prefix at most 2^30 tokens of table (else HFK_ERR_TOO_LARGE); the cache itself may be of any size.
  */
 HFK_API int hfk_prompt_attention_workspace(const hfk_attention* a, uint64_t n_seqs, uint64_t table_width,
                                            uint64_t* bytes);

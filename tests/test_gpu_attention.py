@@ -342,3 +342,30 @@ def test_a_cache_of_more_than_4_gib(cache_kind):
         with pytest.raises(RuntimeError, match="exceeds"):
             ops.prompt_attention(q.to(DEV), k.view(1, blocks * T, H, D), v.view(1, blocks * T, H, D), table[:, :1].to(DEV),
                                  torch.tensor([0, n], device=DEV), torch.tensor([n], device=DEV), out, 0.1)
+
+
+@pytest.mark.parametrize("rows", [1, 3, 20])
+def test_infinite_values_that_are_seen(rows):
+    """An infinity in V gives infinity in its column, whatever the weight's rounding, in every kernel a row can go through."""
+    announce("infinite values, %d rows" % rows)
+    T, D, n = 16, 64, 40
+    gen = torch.Generator().manual_seed(rows)
+    k, v = (torch.randn(4, T, 1, D, generator=gen).to(BF16) for _ in "kv")
+    v[0, 0, 0, 5], v[1, 3, 0, 9], v[2, 1, 0, 9] = float("inf"), float("-inf"), float("inf")
+    k, v = k.to(DEV), v.to(DEV)
+    table = torch.arange(4)[None].to(DEV)
+    q = torch.randn(rows, 4, D, generator=gen).to(BF16).to(DEV)
+    want = torch.zeros(D)
+    want[5], want[9] = float("inf"), float("nan")
+    lens = torch.full((rows,), n, device=DEV)
+    none = torch.zeros(rows, dtype=torch.int64, device=DEV)
+    out = [torch.zeros_like(q) for _ in range(4)]
+    ops.prompt_attention(q, k, v, table, torch.tensor([0, rows], device=DEV), lens[:1], out[0], 0.125, False)
+    ops.prefix_attention(q, k, v, table[0, :0], none[:1], table.repeat(rows, 1), lens, out[1], 0.125)
+    ops.prefix_attention(q, k, v, table[0], lens[:1], table[:, :0].repeat(rows, 1), none, out[2], 0.125)
+    many = table.repeat(1, 40)      # the same blocks again and again: many tiles, splits
+    ops.prompt_attention(q, k, v, many, torch.tensor([0, rows], device=DEV), torch.tensor([160 * T], device=DEV), out[3], 0.125, False)
+    for i, o in enumerate(out):
+        o = o.cpu().float()
+        assert bool((torch.isnan(o) == torch.isnan(want)).all()), i
+        assert bool(((o == float("inf")) == (want == float("inf"))).all()) and not bool((o == float("-inf")).any()), i

@@ -245,7 +245,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(const A
     __shared__ __align__(16) char v_lds[3 * kValueStage];
     __shared__ TileKeys<KEYS> keys[kRing];
     __shared__ TileScales<FP8 ? KEYS : 1> scales[kRing];
-    __shared__ uint32_t not_finite;
+    __shared__ uint32_t not_finite[2];                                    // first and last tile that values were taken out of
 
     const uint32_t tid = threadIdx.x, lane = tid % 64u, wave = __builtin_amdgcn_readfirstlane(tid / 64u), col = lane % 32u, half = lane / 32u;
     const uint32_t head = blockIdx.x % a.cache_heads, rest = blockIdx.x / a.cache_heads;
@@ -415,7 +415,10 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(const A
             }
             *reinterpret_cast<u32x4*>(to + key * kValueRow<DP> + at * 16u) = x;
         });
-        if (found) not_finite = 1u;
+        if (found) {
+            atomicMin(&not_finite[0], tile);
+            atomicMax(&not_finite[1], tile);
+        }
     };
 
     // Where this lane reads in a stage.
@@ -510,7 +513,10 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(const A
     // (second product of tile i - 1, first product of tile i) the other takes weights on the vector units and moves tiles,
     // then a barrier swaps them. The second half starts one barrier late. A tile is put into its stage by both halves'
     // threads one turn before the first half reads it; the stage, one of three, was last read two turns earlier.
-    if (tid == 0) not_finite = 0u;
+    if (tid == 0) {
+        not_finite[0] = ~0u;
+        not_finite[1] = 0u;
+    }
     if (n_tiles == 1) {      // nothing to overlap with, and nothing to load ahead: a short prompt's latency
         if (wave == 0) put_keys(0, load_entry(0));
         __syncthreads();
@@ -632,17 +638,19 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(const A
         }
     }
 
-    // Rare and slow: what was taken out of V, to every row that sees the key it belongs to.
+    // Rare and slow: what was taken out of V, to every row that sees the key it belongs to. Sums of values that are no
+    // numbers do not change when one of them comes twice, so that tiles between these that nothing was taken out of do no harm.
     __syncthreads();
-    if (n_tiles == 0 || not_finite == 0) return;
-    const uint32_t whole = tile_least > first_key ? (tile_least - first_key) / KEYS * KEYS : 0u;    // keys of untouched tiles
+    if (n_tiles == 0 || not_finite[0] == ~0u) return;
+    const uint32_t from_key = first_key + not_finite[0] * KEYS, past = first_key + (not_finite[1] + 1u) * KEYS;
     for (uint32_t n = tid; n < kRows * a.dim; n += kThreads) {
         const uint32_t r = t.first_row + n / a.dim, d = n % a.dim;
         if (r >= n_tile_rows) break;
         const uint32_t of = r / a.group, of_head = head * a.group + r % a.group;
-        const uint32_t until = (uint32_t)seen_by(of) < end_key ? (uint32_t)seen_by(of) : end_key;
+        uint32_t until = (uint32_t)seen_by(of) < end_key ? (uint32_t)seen_by(of) : end_key;
+        until = until < past ? until : past;
         float add = 0.0f;
-        for (uint32_t key = first_key + whole; key < until; ++key) {
+        for (uint32_t key = from_key; key < until; ++key) {
             const uint32_t block = a.split.block32(key), at = key - block * a.split.T;
             const int64_t entry = table[block];
             if ((uint64_t)entry >= a.blocks) continue;
@@ -654,8 +662,12 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(const A
         }
         if (add == 0.0f) continue;
         const uint64_t at_token = t.first_token + of;
-        if (w.to.sum != nullptr) w.to.sum[((uint64_t)split * a.n_rows * heads + at_token * heads + of_head) * a.dim + d] = add;
-        else reinterpret_cast<uint16_t*>(a.out + (int64_t)at_token * a.out_token + (int64_t)of_head * a.out_head)[d] = (uint16_t)T::pack2(add, add);
+        if (w.to.sum != nullptr) {
+            w.to.sum[((uint64_t)split * a.n_rows * heads + at_token * heads + of_head) * a.dim + d] += add;
+        } else {
+            uint16_t& to = reinterpret_cast<uint16_t*>(a.out + (int64_t)at_token * a.out_token + (int64_t)of_head * a.out_head)[d];
+            to = (uint16_t)T::pack2(T::to_float(to) + add, 0.0f);
+        }
     }
 }
 

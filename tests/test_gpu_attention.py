@@ -369,3 +369,33 @@ def test_infinite_values_that_are_seen(rows):
         o = o.cpu().float()
         assert bool((torch.isnan(o) == torch.isnan(want)).all()), i
         assert bool(((o == float("inf")) == (want == float("inf"))).all()) and not bool((o == float("-inf")).any()), i
+
+
+@pytest.mark.parametrize("rows,keys", [(3, 300), (1, 2900)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_values_that_are_no_numbers_around_a_missing_block(rows, keys, causal):
+    """Keys beside a block that is not there, keys of whole tiles and keys of the last, ragged one: each counts wherever it lies."""
+    announce("no numbers around a missing block, %d rows, %d keys, causal %s" % (rows, keys, causal))
+    T, D = 16, 64
+    n = -(-keys // T)
+    gen = torch.Generator().manual_seed(keys)
+    k, v = (torch.randn(n, T, 1, D, generator=gen).to(BF16) for _ in "kv")
+    inf, nan = float("inf"), float("nan")
+    odd = v.clone()
+    for token, column, value in ((5, 4, inf), (5, 3, inf), (130, 3, nan), (130, 7, inf), (keys - rows, 6, -inf), (keys - rows, 8, inf), (50, 8, -inf)):
+        odd[token // T, token % T, 0, column] = value
+    want = {3: nan, 4: inf, 6: -inf, 7: inf, 8: nan}
+    table = torch.arange(n)[None].clone()
+    table[0, 2] = -1
+    table = table.to(DEV)
+    q = torch.randn(rows, 2, D, generator=gen).to(BF16).to(DEV)
+    clean, out = torch.zeros_like(q), torch.zeros_like(q)
+    for values, to in ((v, clean), (odd, out)):
+        ops.prompt_attention(q, k.to(DEV), values.to(DEV), table, torch.tensor([0, rows], device=DEV), torch.tensor([keys], device=DEV), to, 0.125, causal)
+    clean, out = clean.cpu(), out.cpu().float()
+    for column in range(D):
+        got = out[:, :, column]
+        if column not in want:
+            assert torch.equal(got, clean[:, :, column].float()), column
+        else:
+            assert torch.equal(got, torch.full_like(got, want[column])) or bool(torch.isnan(got).all()) and want[column] != want[column], (column, got)

@@ -40,6 +40,17 @@ void check_written(const at::Tensor& t, const char* what) {
     TORCH_CHECK(at::has_internal_overlap(t) != at::MemOverlap::Yes, what, " is written and must not overlap itself");
 }
 
+// Two tensors of which at least one is written; views whose overlap cannot be told at a glance are the caller's.
+void check_apart(const at::Tensor& a, const at::Tensor& b, const char* what, bool same_allowed = false) {
+    const at::MemOverlapStatus s = at::get_overlap_status(a, b);
+    TORCH_CHECK(s != at::MemOverlapStatus::Partial && (same_allowed || s != at::MemOverlapStatus::Full), what, " must not overlap");
+}
+
+void check_no_gradient(const at::Tensor& t, const char* what) {
+    TORCH_CHECK(!(at::GradMode::is_enabled() && t.requires_grad()), what,
+                " requires a gradient, which this op does not compute: detach it or call the op under torch.no_grad()");
+}
+
 void check_index(const at::Tensor& t, const at::Tensor& cache, int64_t dims, const char* what) {
     check_on(t, cache, what);
     TORCH_CHECK(t.scalar_type() == at::kLong, what, " must be int64");
@@ -135,6 +146,14 @@ void cache_write(const at::Tensor& k, const at::Tensor& kCache, const at::Tensor
     if (kScales.has_value()) check_written(*kScales, "kScales");
     if (t.both) check_written(*vCache, "vCache");
     if (vScales.has_value()) check_written(*vScales, "vScales");
+    check_no_gradient(k, "k");
+    check_no_gradient(kCache, "kCache");
+    if (t.both) {
+        check_no_gradient(*v, "v");
+        check_no_gradient(*vCache, "vCache");
+        check_apart(kCache, *vCache, "kCache and vCache");
+        if (vScales.has_value()) check_apart(*kScales, *vScales, "kScales and vScales");
+    }
     const c10::hip::OptionalHIPGuardMasqueradingAsCUDA device_guard(device_of(kCache));
     check_call(hfk_cache_write(&t.plane[0], &t.rows[0], t.both ? &t.plane[1] : nullptr, t.both ? &t.rows[1] : nullptr,
                                slots.data_ptr<int64_t>(), static_cast<uint64_t>(t.n), stream_of_current_device()),
@@ -146,7 +165,14 @@ void cache_read(const at::Tensor& kCache, const at::Tensor& k, const at::Tensor&
                 const OptTensor& kScales, const OptTensor& vScales) {
     const Tokens t = tokens_of(k, kCache, slots, v, vCache, kScales, vScales);
     check_written(k, "k");
-    if (t.both) check_written(*v, "v");
+    check_no_gradient(kCache, "kCache");
+    check_no_gradient(k, "k");
+    if (t.both) {
+        check_written(*v, "v");
+        check_no_gradient(*vCache, "vCache");
+        check_no_gradient(*v, "v");
+        check_apart(k, *v, "k and v");
+    }
     const c10::hip::OptionalHIPGuardMasqueradingAsCUDA device_guard(device_of(kCache));
     check_call(hfk_cache_read(&t.plane[0], &t.rows[0], t.both ? &t.plane[1] : nullptr, t.both ? &t.rows[1] : nullptr,
                               slots.data_ptr<int64_t>(), static_cast<uint64_t>(t.n), stream_of_current_device()),
@@ -167,6 +193,11 @@ hfk_attention attention_of(const at::Tensor& q, const at::Tensor& kCache, const 
     a.q = rows_of(q, kCache, q.size(0), q.size(1), "q");
     a.out = rows_of(out, kCache, q.size(0), q.size(1), "out");
     check_written(out, "out");
+    check_apart(out, q, "out and q, unless they are one tensor,", true);
+    check_no_gradient(q, "q");
+    check_no_gradient(kCache, "kCache");
+    check_no_gradient(vCache, "vCache");
+    check_no_gradient(out, "out");
     TORCH_CHECK(q.size(1) > 0 && q.size(1) <= 0xffffffffLL && q.size(1) % kCache.size(2) == 0, "q has ", q.size(1),
                 " heads, which is no multiple of the cache's ", kCache.size(2));
     TORCH_CHECK(out.scalar_type() == q.scalar_type(), "out must have q's type");
@@ -175,7 +206,7 @@ hfk_attention attention_of(const at::Tensor& q, const at::Tensor& kCache, const 
     a.n_rows = static_cast<uint64_t>(q.size(0));
     a.q_heads = static_cast<uint32_t>(q.size(1));
     a.scale = static_cast<float>(scale);
-    TORCH_CHECK(a.scale > 0.0f && a.scale <= 3.402823466e38f, "scale must be positive and finite, got ", scale);
+    TORCH_CHECK(a.scale >= 0x1p-100f && a.scale <= 0x1p100f, "scale must be positive and finite, from 2^-100 to 2^100, got ", scale);
     if (lse.has_value()) {
         check_on(*lse, kCache, "lse");
         TORCH_CHECK(lse->scalar_type() == at::kFloat && lse->is_contiguous() && lse->dim() == 2 && lse->size(0) == q.size(0) &&

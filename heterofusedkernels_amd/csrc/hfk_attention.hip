@@ -1202,7 +1202,7 @@ int check_attention(const hfk_attention* a) {
     if (k.blocks != v.blocks || k.block_tokens != v.block_tokens || k.heads != v.heads || k.head_dim != v.head_dim) return HFK_ERR_BAD_SIZE;
     if (k.head_dim % 16u != 0 || k.head_dim > 256u) return HFK_ERR_BAD_SIZE;
     if (a->q_heads == 0 || a->q_heads % k.heads != 0) return HFK_ERR_BAD_SIZE;
-    if (!(a->scale > 0.0f) || !std::isfinite(a->scale)) return HFK_ERR_BAD_SIZE;
+    if (!(a->scale >= 0x1p-100f && a->scale <= 0x1p100f)) return HFK_ERR_BAD_SIZE;      // kLazily / scale stays finite, too
     if (a->q_heads > 65535u || a->n_rows > 0x7fffffffull || a->n_rows * a->q_heads > 0x7fffffffull) return HFK_ERR_TOO_LARGE;
     if (!block_fits(k) || !block_fits(v)) return HFK_ERR_TOO_LARGE;
     if (!hfk::plane_aligned(k, 16) || !hfk::plane_aligned(v, 16) || !hfk::rows_aligned(a->q) || !hfk::rows_aligned(a->out))

@@ -484,7 +484,8 @@ typedef struct hfk_token_rows {
  *     A power of two makes the division, and the product on the way back, exact: the only error is
  *     the rounding to 4 significant bits.
  * v_plane and v may both be NULL (a cache of one latent tensor per layer); the two sides may differ
- * in heads and head_dim. slots are device-visible; slots of one call must be distinct.
+ * in heads and head_dim. slots are device-visible; slots of one call must be distinct: of two rows for one slot
+ * any mixture may be left there, values of one under the scale of the other included.
  * Any head_dim up to 1024 and any strides; rows and planes whose pointers and strides are multiples of
  * 16 bytes (8 for the HFK_FP8_E4M3 side) with head_dim a multiple of 8 take the vectorised path.
  */
@@ -503,11 +504,12 @@ HFK_API int hfk_cache_read(const hfk_cache_plane* k_plane, const hfk_token_rows*
 /* Queries and results of one attention call. */
 typedef struct hfk_attention {
     hfk_cache_plane k, v;        /* same blocks, block_tokens, heads, head_dim and type */
-    hfk_token_rows q, out;       /* n_rows tokens of q_heads heads of head_dim values, of one type */
+    hfk_token_rows q, out;       /* n_rows tokens of q_heads heads of head_dim values, of one type; out may be q itself,
+                                    and overlaps it in no other way */
     float* lse;                  /* [n_rows][q_heads] natural logarithm of each row's sum of exponentials, or NULL */
     uint64_t n_rows;
     uint32_t q_heads;            /* a multiple of k.heads: query head h reads cache head h / (q_heads / k.heads) */
-    float scale;                 /* of the scores, positive and finite */
+    float scale;                 /* of the scores, from 2^-100 to 2^100 */
 } hfk_attention;
 
 /*

@@ -191,3 +191,12 @@ def test_plain_quantiser_follows_its_definition():
     y = torch.randn(50, 64, generator=gen)
     q, s = quantise(y)
     assert bool(((dequantise(q, s, torch.float32) - y).abs() <= y.abs() * 2.0 ** -4 + s[:, None] * 2.0 ** -10).all())
+
+
+def test_scales_of_scores_beyond_the_range_are_refused():
+    """At its ends the running maximum's threshold, or the scale in base 2, would leave 32 bits."""
+    for scale in (1e-39, 2.0 ** -101, 2.0 ** 101, 3e38):
+        assert capi.prompt_attention_workspace(attention(scale=scale), 1, 4)[0] == -2
+        assert capi.prefix_attention_workspace(attention(scale=scale), 4, 4)[0] == -2
+    for scale in (2.0 ** -100, 2.0 ** 100):
+        assert capi.prompt_attention_workspace(attention(scale=scale), 1, 4)[0] == 0

@@ -262,6 +262,49 @@ def test_refusals():
     torch.cuda.synchronize()
 
 
+def test_refusals_of_overlaps_and_gradients():
+    """Two written sides in one memory, results half in the queries, gradients that nobody would compute."""
+    announce("refusals of overlaps and gradients")
+    k = torch.zeros(4, 16, 2, 64, dtype=BF16, device=DEV)
+    f, fs = torch.zeros(4, 16, 2, 64, dtype=FP8, device=DEV), torch.ones(4, 16, 2, device=DEV)
+    x, slots = torch.zeros(4, 2, 64, dtype=BF16, device=DEV), torch.arange(3, device=DEV)
+    with pytest.raises(RuntimeError, match="kCache and vCache must not overlap"):
+        ops.cache_write(x[:3], k, slots, x[:3], k)
+    with pytest.raises(RuntimeError, match="kScales and vScales must not overlap"):
+        ops.cache_write(x[:3], f, slots, x[:3], f.clone(), fs, fs)
+    with pytest.raises(RuntimeError, match="k and v must not overlap"):
+        ops.cache_read(k, x[:3], slots, k, x[1:])
+    q = torch.zeros(4, 4, 64, dtype=BF16, device=DEV)
+    table, starts, lens = torch.zeros(1, 2, dtype=torch.int64, device=DEV), torch.tensor([0, 3], device=DEV), torch.tensor([5], device=DEV)
+    with pytest.raises(RuntimeError, match="out and q, unless they are one tensor, must not overlap"):
+        ops.prompt_attention(q[:3], k, k, table, starts, lens, q[1:], 0.1)
+    with pytest.raises(RuntimeError, match="q requires a gradient"):
+        ops.prompt_attention(q[:3].clone().requires_grad_(), k, k, table, starts, lens, q[:3], 0.1)
+    with pytest.raises(RuntimeError, match="kCache requires a gradient"):
+        ops.prefix_attention(q, k.clone().requires_grad_(), k, table[0], lens, table.repeat(4, 1), lens.repeat(4), q, 0.1)
+    with pytest.raises(RuntimeError, match="v requires a gradient"):
+        ops.cache_write(x[:3], k, slots, x[:3].clone().requires_grad_(), k.clone())
+    with torch.no_grad():
+        ops.prompt_attention(q[:3].clone().requires_grad_(), k, k, table, starts, lens, q[:3], 0.1)
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("rows,keys", [(300, 300), (5, 40), (5, 2000)])
+def test_results_in_place_of_the_queries(rows, keys):
+    announce("results in place of the queries, %d rows, %d keys" % (rows, keys))
+    gen = torch.Generator().manual_seed(rows)
+    k, v = (torch.randn(-(-keys // 16), 16, 2, 64, generator=gen).to(BF16).to(DEV) for _ in "kv")
+    q = torch.randn(rows, 8, 64, generator=gen).to(BF16).to(DEV)
+    table = torch.arange(len(k), device=DEV)[None]
+    starts, lens = torch.tensor([0, rows], device=DEV), torch.tensor([keys], device=DEV)
+    want = [torch.empty_like(q) for _ in range(2)]
+    got = [q.clone() for _ in range(2)]
+    for to, of in zip((want, got), ([q, q], got)):
+        ops.prompt_attention(of[0], k, v, table, starts, lens, to[0], 0.125)
+        ops.prefix_attention(of[1], k, v, table[0, :2], lens.clamp(max=20), table.repeat(rows, 1), lens.repeat(rows), to[1], 0.125)
+    assert same(got, want)
+
+
 def test_refused_calls_have_no_effect_and_capture_goes_on():
     """A refused call inside a capture leaves the capture sound."""
     announce("a refusal inside a capture")

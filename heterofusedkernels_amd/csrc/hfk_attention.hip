@@ -745,7 +745,7 @@ __device__ bool find_range(const NarrowWalk& w, uint32_t T, uint32_t range, uint
 // HEADS == 4: a wave for each of four neighbouring cache heads, all at the same keys. HEADS == 1: four waves at one head, whose
 // sums meet in LDS.
 template <typename T, bool FP8, int DP, int R, int HEADS>
-__global__ __launch_bounds__(256, R * DP <= 256 ? 2 : 1) void narrow_attention_kernel(const AttentionArgs a, const NarrowWalk prefix, const NarrowWalk own) {
+__global__ __launch_bounds__(256, R * DP <= 256 && DP != 256 ? 2 : 1) void narrow_attention_kernel(const AttentionArgs a, const NarrowWalk prefix, const NarrowWalk own) {
     constexpr int kKSteps = DP / 32;        // matrix instructions of the first product
     constexpr int kCols = DP / 16;          // values of V per lane and key
     constexpr uint32_t kRegs = R * kCols * 4, kWavesPerHead = 4 / HEADS, kUnit = kWavesPerHead * 32;

@@ -61,7 +61,9 @@ inline NarrowPlan plan_narrow(uint64_t rows, uint32_t cache_heads, uint32_t head
     const uint32_t dim = padded_head_dim(head_dim), most = dim == 256 ? 2 : 4;
     p.row_blocks = rows <= 16 ? 1 : (rows <= 32 || most == 2) ? 2 : 4;
     p.row_tiles = ceil_div(rows, 16ull * p.row_blocks);
-    const uint64_t resident = p.row_blocks * dim <= 256 ? 512 : 256, same_keys = p.row_tiles * (cache_heads / narrow_heads(cache_heads));
+    // Two per compute unit where their registers fit without spilling. (24 sequences of 8000 tokens, 4 heads of 256 in bf16: 149 us
+    // with one, 180 with two whose registers spill; one sequence of 32000: 44 and 67 us.)
+    const uint64_t resident = p.row_blocks * dim <= 256 && dim != 256 ? 512 : 256, same_keys = p.row_tiles * (cache_heads / narrow_heads(cache_heads));
     uint64_t ranges = min64(max64(1, resident / same_keys), max64(1, units));
     if (ranges > 8) ranges -= ranges % 8;      // the same number for each XCD
     p.ranges = (uint32_t)ranges;

@@ -766,11 +766,12 @@ __global__ __launch_bounds__(256, R * DP <= 256 && DP != 256 ? 2 : 1) void narro
     constexpr bool kRest = R * DP <= 128;
     constexpr int kRowPieces = FP8 ? DP / 16 : DP / 8;                   // 16-byte pieces of a cached row
     constexpr uint32_t kRowBytes = kRowPieces * 16 + 16;                 // of K in LDS: 16 rows' pieces of one column, no bank twice
-    struct WaveLds {                                                     // a wave's own: no barrier, LDS serves a wave in order
+    struct alignas(16) WaveLds {                                         // a wave's own: no barrier, LDS serves a wave in order
         char k[32 * kRowBytes];
         int64_t place[32][2];                                            // of a key's K and V
         float scale[2][FP8 ? 32 : 1];
     };
+    static_assert(alignof(WaveLds) == 16 && sizeof(WaveLds) % 16 == 0);  // every wave's K is written and read 16 bytes at a time
     __shared__ float tops[4][R * 16], sums[4][R * 16];
     __shared__ __align__(16) union {
         WaveLds wave[4];

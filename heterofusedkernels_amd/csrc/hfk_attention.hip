@@ -336,7 +336,9 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(const A
     // Which keys of a tile are visible, as a scalar.
     constexpr uint64_t kAll = KEYS == 64 ? ~0ull : (1ull << (KEYS % 64)) - 1ull;
     const auto as_scalar = [](uint64_t x) -> uint64_t {
-        return (uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(x >> 32)) << 32 | __builtin_amdgcn_readfirstlane((uint32_t)x);
+        // (the builtin gives an int: a half that begins with a one must not be extended by its sign)
+        const uint32_t high = __builtin_amdgcn_readfirstlane((uint32_t)(x >> 32)), low = __builtin_amdgcn_readfirstlane((uint32_t)x);
+        return (uint64_t)high << 32 | low;
     };
     // A tile's keys, or its values, into registers and from there into their stage. A thread has the same piece of every
     // row it moves; pieces beyond head_dim stay zero.

@@ -871,7 +871,11 @@ __global__ __launch_bounds__(256, R * DP <= 256 && DP != 256 ? 2 : 1) void narro
             const bool ok = key < end_key && (uint64_t)entry < a.blocks;
             x.seen = (uint32_t)__ballot(ok);
             const uint32_t block = ok ? (uint32_t)entry : 0u, at = ok ? key - a.split.block32(key) * a.split.T : 0u;
-            if constexpr (FP8) x.scale = lane < 32u ? k_scale_base[scale_place(a.k, block, at)] : v_scale_base[scale_place(a.v, block, at)];
+            // (a scale of a key that is not visible may be anything, and one that is no number makes NaN even of a zero)
+            if constexpr (FP8) {
+                const float scale = lane < 32u ? k_scale_base[scale_place(a.k, block, at)] : v_scale_base[scale_place(a.v, block, at)];
+                x.scale = ok ? scale : 1.0f;
+            }
             mine.place[lane % 32u][lane / 32u] = lane < 32u ? place(a.k, block, at) : place(a.v, block, at);
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             for (int n = 0; n < kLoads; ++n) {

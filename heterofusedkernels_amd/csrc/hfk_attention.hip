@@ -1130,7 +1130,9 @@ __global__ __launch_bounds__(256) void join_splits_kernel(const AttentionArgs a,
     const uint32_t lanes = a.dim <= 64u ? 16u : a.dim <= 128u ? 32u : 64u, side_by_side = 64u / lanes;
     const uint32_t d = lane % lanes * 4u, mine = lane / lanes;
     // One pass: 64 splits' statistics at a time, a running maximum, and four loads of sums in flight that wait for no weight. A
-    // split whose weight is zero may hold anything, or nothing written: it is read and not used.
+    // split that saw nothing has no sum written: what lies there is read and not used, as its weight kUnseen says. A weight that is
+    // zero in 32 bits only still multiplies: NaN among a split's sums stays NaN whatever the other splits hold.
+    constexpr float kUnseen = -1.0f;
     float high = kMinusInf, total = 0.0f;
     f32x4 acc{0, 0, 0, 0};
     for (uint32_t base = wave * 64u; base < splits; base += 64u * WAVES) {
@@ -1158,15 +1160,15 @@ __global__ __launch_bounds__(256) void join_splits_kernel(const AttentionArgs a,
             total *= keep;
             high = most;
         }
-        const float weight = top == kMinusInf ? 0.0f : __builtin_amdgcn_exp2f(top - high);
-        total += weight == 0.0f ? 0.0f : weight * sum;
+        const float weight = top == kMinusInf ? kUnseen : __builtin_amdgcn_exp2f(top - high);
+        total += weight == kUnseen ? 0.0f : weight * sum;
         for (uint32_t s = 0; s < n; s += 4u * side_by_side) {
             if (s != 0) load_sums(s, x);
             for (uint32_t i = 0; i < 4u; ++i) {
                 const uint32_t from = s + i * side_by_side + mine;
                 float by = __shfl(weight, (int)(from & 63u));              // by all lanes, whether they have such a split or not
-                if (from >= n) by = 0.0f;
-                for (int c = 0; c < 4; ++c) acc[c] += by == 0.0f ? 0.0f : by * x[i][c];
+                if (from >= n) by = kUnseen;
+                for (int c = 0; c < 4; ++c) acc[c] += by == kUnseen ? 0.0f : by * x[i][c];
             }
         }
     }

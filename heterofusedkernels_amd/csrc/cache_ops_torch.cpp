@@ -130,7 +130,9 @@ Tokens tokens_of(const at::Tensor& k, const at::Tensor& kCache, const at::Tensor
     t.both = v.has_value();
     if (t.both) {
         check_on(*vCache, kCache, "vCache");
-        t.plane[1] = plane_of(*vCache, vScales, "vCache");
+        TORCH_CHECK(vCache->scalar_type() == kCache.scalar_type(), "kCache and vCache must have one type, got ",
+                    c10::toString(kCache.scalar_type()), " and ", c10::toString(vCache->scalar_type()));
+        t.plane[1] = plane_of(*vCache, vScales, "vCache");      // so that both have scales or neither has
         t.rows[1] = rows_of(*v, *vCache, t.n, vCache->size(2), "v");
     }
     return t;

@@ -1208,7 +1208,9 @@ constexpr uint64_t kMostKeys = 1ull << 30;       // of one sequence
 // Products of a block's stride, and of a token's inside its block, fit 32 bits.
 bool block_fits(const hfk_cache_plane& p) {
     const uint64_t e = hfk::type_bytes(p.type), most = 0xffffffffull;
-    const auto fits = [&](uint64_t block, uint64_t token) { return (p.blocks <= 1 || block <= most) && token * (p.block_tokens - 1) <= most; };
+    const auto fits = [&](uint64_t block, uint64_t token) {      // by division: a product of the two passes 64 bits, too
+        return (p.blocks <= 1 || block <= most) && (p.block_tokens == 1 || token <= most / (p.block_tokens - 1));
+    };
     return fits(e * (uint64_t)p.block_stride, e * (uint64_t)p.token_stride) &&
            (p.type != HFK_FP8_E4M3 || fits((uint64_t)p.scale_block_stride, (uint64_t)p.scale_token_stride));
 }

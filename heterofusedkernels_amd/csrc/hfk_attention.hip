@@ -1371,7 +1371,7 @@ int hfk_prompt_attention(const hfk_attention* a, const int64_t* block_table, uin
     const hfk::PromptPlan p = hfk::plan_prompt(a->n_rows, a->q_heads, a->k.heads, a->k.head_dim, n_seqs, keys);
     rc = check_workspace(workspace, workspace_bytes, p.workspace);
     if (rc != HFK_OK) return rc;
-    if (p.wide.groups > 0x7fffffffull) return HFK_ERR_TOO_LARGE;
+    if (!hfk::launch_fits(p.wide.groups, kWideThreads)) return HFK_ERR_TOO_LARGE;
     const AttentionArgs x = fill(a);
     WideWalk w{};
     w.table = block_table;
@@ -1427,7 +1427,9 @@ int hfk_prefix_attention(const hfk_attention* a, const int64_t* prefix_blocks, u
     const hfk::PrefixPlan p = hfk::plan_prefix(a->n_rows, a->q_heads, a->k.heads, a->k.head_dim, prefix, own);
     rc = check_workspace(workspace, workspace_bytes, p.workspace);
     if (rc != HFK_OK) return rc;
-    if (p.wide.groups + p.prefix.groups + p.own.groups > 0x7fffffffull || a->n_rows * hfk::ceil_div(own, hfk::narrow_unit(a->k.heads)) > 0x7fffffffull)
+    if (!hfk::launch_fits(p.wide.groups, kWideThreads) || !hfk::launch_fits(p.prefix.groups + p.own.groups, 256) ||
+        !hfk::launch_fits(hfk::ceil_div(a->n_rows * a->q_heads, 4), 256) ||
+        a->n_rows * hfk::ceil_div(own, hfk::narrow_unit(a->k.heads)) > 0x7fffffffull)
         return HFK_ERR_TOO_LARGE;
     const AttentionArgs x = fill(a);
     const bool narrow_prefix = prefix != 0 && !p.wide_prefix;

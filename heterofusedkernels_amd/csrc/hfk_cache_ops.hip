@@ -365,7 +365,7 @@ int move_tokens(const hfk_cache_plane* kp, const hfk_token_rows* k, const hfk_ca
         const uint32_t its = (s.dim + s.lanes * piece - 1u) / (s.lanes * piece);
         if (its > chunks) chunks = its;
     }
-    if (groups[0] + groups[1] > 0x7fffffffull) return HFK_ERR_TOO_LARGE;
+    if (!hfk::launch_fits(groups[0] + groups[1], 256)) return HFK_ERR_TOO_LARGE;
     a.first_groups = (uint32_t)groups[0];
     const uint32_t grid = (uint32_t)(groups[0] + groups[1]);
     hipStream_t s = static_cast<hipStream_t>(stream);

@@ -94,6 +94,9 @@ inline bool multiple_of(const void* p, uint64_t n) { return (uint64_t)(uintptr_t
 // products inside 64 bits.
 inline bool stride_fits(int64_t s) { return s >= 0 && s < (1ll << 40); }
 
+// A launch's threads are counted in 32 bits.
+inline bool launch_fits(uint64_t groups, uint32_t threads) { return groups * threads < (1ull << 32); }
+
 inline int check_plane(const hfk_cache_plane& p) {
     if (!known_type(p.type)) return HFK_ERR_BAD_TYPE;
     if (p.block_tokens == 0 || p.heads == 0 || p.head_dim == 0) return HFK_ERR_BAD_SIZE;

@@ -487,7 +487,8 @@ typedef struct hfk_token_rows {
  * in heads and head_dim. slots are device-visible; slots of one call must be distinct: of two rows for one slot
  * any mixture may be left there, values of one under the scale of the other included.
  * Any head_dim up to 1024 and any strides; rows and planes whose pointers and strides are multiples of
- * 16 bytes (8 for the HFK_FP8_E4M3 side) with head_dim a multiple of 8 take the vectorised path.
+ * 16 bytes (8 for the HFK_FP8_E4M3 side) with head_dim a multiple of 8 take the vectorised path. A call whose launch would
+ * have 2^32 threads is HFK_ERR_TOO_LARGE: 2^28 rows (a token's head) of 128 values in 16 bits.
  */
 HFK_API int hfk_cache_write(const hfk_cache_plane* k_plane, const hfk_token_rows* k, const hfk_cache_plane* v_plane,
                             const hfk_token_rows* v, const int64_t* slots, uint64_t n, hfk_stream_t stream);
@@ -532,7 +533,8 @@ typedef struct hfk_attention {
  * and sums are held in 32 bits. The second product takes the weights in q's type; where a launch waits for
  * memory (few rows per cache head, head_dim up to 128) it takes their rounding error too, as a second operand.
  * head_dim: a multiple of 16 up to 256. All pointers and strides multiples of 16 bytes. A block spans less than
- * 4 GiB and a sequence or the prefix at most 2^30 tokens of table (else HFK_ERR_TOO_LARGE); the cache itself may be of any size.
+ * 4 GiB, a sequence or the prefix has at most 2^30 tokens of table, and no launch has 2^32 threads (n_rows * q_heads / 256 + n_seqs * heads below
+ * 2^23 for prompts, n_rows * q_heads below 2^26 for hfk_prefix_attention), else HFK_ERR_TOO_LARGE; the cache itself may be of any size.
  */
 HFK_API int hfk_prompt_attention_workspace(const hfk_attention* a, uint64_t n_seqs, uint64_t table_width,
                                            uint64_t* bytes);

@@ -8,6 +8,7 @@
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <torch/library.h>
 
+#include <initializer_list>
 #include <optional>
 
 #include "hfk.h"
@@ -40,10 +41,37 @@ void check_written(const at::Tensor& t, const char* what) {
     TORCH_CHECK(at::has_internal_overlap(t) != at::MemOverlap::Yes, what, " is written and must not overlap itself");
 }
 
-// Two tensors of which at least one is written; views whose overlap cannot be told at a glance are the caller's.
-void check_apart(const at::Tensor& a, const at::Tensor& b, const char* what, bool same_allowed = false) {
-    const at::MemOverlapStatus s = at::get_overlap_status(a, b);
-    TORCH_CHECK(s != at::MemOverlapStatus::Partial && (same_allowed || s != at::MemOverlapStatus::Full), what, " must not overlap");
+// An argument and the bytes from its first value to its last one; none where it is not given or empty.
+struct Named {
+    const at::Tensor* tensor = nullptr;
+    const char* name;
+    uintptr_t first = 0, end = 0;
+    Named(const at::Tensor& t, const char* name) : tensor(&t), name(name) {
+        if (t.numel() == 0) return;
+        const at::IntArrayRef sizes = t.sizes(), strides = t.strides();
+        int64_t last = 0;
+        for (size_t i = 0; i < sizes.size(); ++i) last += (sizes[i] - 1) * strides[i];
+        first = reinterpret_cast<uintptr_t>(t.const_data_ptr());
+        end = first + static_cast<uintptr_t>(last + 1) * t.element_size();
+    }
+    Named(const OptTensor& t, const char* name) : name(name) {
+        if (t.has_value()) *this = Named(*t, name);
+    }
+};
+
+// What is written lies apart from everything else that is written and from everything that is read: rows are read and written
+// by different workgroups in no order. Views whose overlap cannot be told at a glance are the caller's. (Most pairs are apart by their
+// addresses, which costs a call of one token 0.1 us; at::get_overlap_status for each of them 0.3.)
+void check_apart(std::initializer_list<Named> written, std::initializer_list<Named> read) {
+    const auto check = [](const Named& a, const Named& b) {
+        if (a.first >= b.end || b.first >= a.end) return;
+        const at::MemOverlapStatus s = at::get_overlap_status(*a.tensor, *b.tensor);
+        TORCH_CHECK(s != at::MemOverlapStatus::Partial && s != at::MemOverlapStatus::Full, a.name, " and ", b.name, " must not overlap");
+    };
+    for (const Named* w = written.begin(); w != written.end(); ++w) {
+        for (const Named* other = w + 1; other != written.end(); ++other) check(*w, *other);
+        for (const Named& r : read) check(*w, r);
+    }
 }
 
 void check_no_gradient(const at::Tensor& t, const char* what) {
@@ -153,9 +181,9 @@ void cache_write(const at::Tensor& k, const at::Tensor& kCache, const at::Tensor
     if (t.both) {
         check_no_gradient(*v, "v");
         check_no_gradient(*vCache, "vCache");
-        check_apart(kCache, *vCache, "kCache and vCache");
-        if (vScales.has_value()) check_apart(*kScales, *vScales, "kScales and vScales");
     }
+    check_apart({{kCache, "kCache"}, {vCache, "vCache"}, {kScales, "kScales"}, {vScales, "vScales"}},
+                {{k, "k"}, {v, "v"}, {slots, "slots"}});
     const c10::hip::OptionalHIPGuardMasqueradingAsCUDA device_guard(device_of(kCache));
     check_call(hfk_cache_write(&t.plane[0], &t.rows[0], t.both ? &t.plane[1] : nullptr, t.both ? &t.rows[1] : nullptr,
                                slots.data_ptr<int64_t>(), static_cast<uint64_t>(t.n), stream_of_current_device()),
@@ -173,8 +201,9 @@ void cache_read(const at::Tensor& kCache, const at::Tensor& k, const at::Tensor&
         check_written(*v, "v");
         check_no_gradient(*vCache, "vCache");
         check_no_gradient(*v, "v");
-        check_apart(k, *v, "k and v");
     }
+    check_apart({{k, "k"}, {v, "v"}},
+                {{kCache, "kCache"}, {vCache, "vCache"}, {kScales, "kScales"}, {vScales, "vScales"}, {slots, "slots"}});
     const c10::hip::OptionalHIPGuardMasqueradingAsCUDA device_guard(device_of(kCache));
     check_call(hfk_cache_read(&t.plane[0], &t.rows[0], t.both ? &t.plane[1] : nullptr, t.both ? &t.rows[1] : nullptr,
                               slots.data_ptr<int64_t>(), static_cast<uint64_t>(t.n), stream_of_current_device()),
@@ -195,7 +224,9 @@ hfk_attention attention_of(const at::Tensor& q, const at::Tensor& kCache, const 
     a.q = rows_of(q, kCache, q.size(0), q.size(1), "q");
     a.out = rows_of(out, kCache, q.size(0), q.size(1), "out");
     check_written(out, "out");
-    check_apart(out, q, "out and q, unless they are one tensor,", true);
+    TORCH_CHECK(at::get_overlap_status(out, q) != at::MemOverlapStatus::Partial, "out and q, unless they are one tensor, must not overlap");
+    check_apart({{lse, "lse"}}, {{q, "q"}});
+    check_apart({{out, "out"}, {lse, "lse"}}, {{kCache, "kCache"}, {vCache, "vCache"}, {kScales, "kScales"}, {vScales, "vScales"}});
     check_no_gradient(q, "q");
     check_no_gradient(kCache, "kCache");
     check_no_gradient(vCache, "vCache");
@@ -237,6 +268,7 @@ void prompt_attention(const at::Tensor& q, const at::Tensor& kCache, const at::T
     const int64_t n = kvLens.size(0);
     TORCH_CHECK(blockTable.size(0) == n && queryStarts.size(0) == n + 1, "blockTable must have one row and queryStarts one entry more per kvLens' ",
                 n, " sequences, got ", blockTable.size(0), " and ", queryStarts.size(0));
+    check_apart({{out, "out"}, {lse, "lse"}}, {{blockTable, "blockTable"}, {queryStarts, "queryStarts"}, {kvLens, "kvLens"}});
     const c10::hip::OptionalHIPGuardMasqueradingAsCUDA device_guard(device_of(kCache));
     const uint64_t width = static_cast<uint64_t>(blockTable.size(1));
     uint64_t bytes = 0;
@@ -259,6 +291,8 @@ void prefix_attention(const at::Tensor& q, const at::Tensor& kCache, const at::T
     check_index(kvLens, kCache, 1, "kvLens");
     TORCH_CHECK(prefixLen.size(0) == 1, "prefixLen must hold one length");
     TORCH_CHECK(blockTable.size(0) == q.size(0) && kvLens.size(0) == q.size(0), "blockTable and kvLens must have one row per row of q");
+    check_apart({{out, "out"}, {lse, "lse"}},
+                {{prefixBlocks, "prefixBlocks"}, {prefixLen, "prefixLen"}, {blockTable, "blockTable"}, {kvLens, "kvLens"}});
     const c10::hip::OptionalHIPGuardMasqueradingAsCUDA device_guard(device_of(kCache));
     const uint64_t prefix = static_cast<uint64_t>(prefixBlocks.size(0)), width = static_cast<uint64_t>(blockTable.size(1));
     uint64_t bytes = 0;

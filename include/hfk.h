@@ -486,6 +486,8 @@ typedef struct hfk_token_rows {
  * v_plane and v may both be NULL (a cache of one latent tensor per layer); the two sides may differ
  * in heads and head_dim. slots are device-visible; slots of one call must be distinct: of two rows for one slot
  * any mixture may be left there, values of one under the scale of the other included.
+ * What is written (here planes and scales, in hfk_cache_read the rows) shares no memory with anything else that the call reads or
+ * writes: rows are taken in no order. Tokens move within a cache through hfk_cache_read and rows of their own.
  * Any head_dim up to 1024 and any strides; rows and planes whose pointers and strides are multiples of
  * 16 bytes (8 for the HFK_FP8_E4M3 side) with head_dim a multiple of 8 take the vectorised path. A call whose launch would
  * have 2^32 threads is HFK_ERR_TOO_LARGE: 2^28 rows (a token's head) of 128 values in 16 bits.
@@ -529,6 +531,7 @@ typedef struct hfk_attention {
  *   kv_lens       device int64 [n_seqs]; taken to lie within [0, table_width * T]
  *   workspace     device memory of hfk_prompt_attention_workspace() bytes, 256-byte aligned (NULL if that is 0),
  *                 written and read by this call alone until the stream has passed it
+ * out (unless it is q) and lse share no memory with each other or with anything that is read.
  * Types: q and out HFK_BF16 or HFK_FP16; the cache of the same type or HFK_FP8_E4M3. Scores, statistics
  * and sums are held in 32 bits. The second product takes the weights in q's type; where a launch waits for
  * memory (few rows per cache head, head_dim up to 128) it takes their rounding error too, as a second operand.

@@ -78,6 +78,9 @@ void check_no_gradient(const at::Tensor& t, const char* what) {
     TORCH_CHECK(!(at::GradMode::is_enabled() && t.requires_grad()), what,
                 " requires a gradient, which this op does not compute: detach it or call the op under torch.no_grad()");
 }
+void check_no_gradient(const OptTensor& t, const char* what) {
+    if (t.has_value()) check_no_gradient(*t, what);
+}
 
 void check_index(const at::Tensor& t, const at::Tensor& cache, int64_t dims, const char* what) {
     check_on(t, cache, what);
@@ -163,6 +166,12 @@ Tokens tokens_of(const at::Tensor& k, const at::Tensor& kCache, const at::Tensor
         t.plane[1] = plane_of(*vCache, vScales, "vCache");      // so that both have scales or neither has
         t.rows[1] = rows_of(*v, *vCache, t.n, vCache->size(2), "v");
     }
+    check_no_gradient(k, "k");
+    check_no_gradient(v, "v");
+    check_no_gradient(kCache, "kCache");
+    check_no_gradient(vCache, "vCache");
+    check_no_gradient(kScales, "kScales");
+    check_no_gradient(vScales, "vScales");
     return t;
 }
 
@@ -176,12 +185,6 @@ void cache_write(const at::Tensor& k, const at::Tensor& kCache, const at::Tensor
     if (kScales.has_value()) check_written(*kScales, "kScales");
     if (t.both) check_written(*vCache, "vCache");
     if (vScales.has_value()) check_written(*vScales, "vScales");
-    check_no_gradient(k, "k");
-    check_no_gradient(kCache, "kCache");
-    if (t.both) {
-        check_no_gradient(*v, "v");
-        check_no_gradient(*vCache, "vCache");
-    }
     check_apart({{kCache, "kCache"}, {vCache, "vCache"}, {kScales, "kScales"}, {vScales, "vScales"}},
                 {{k, "k"}, {v, "v"}, {slots, "slots"}});
     const c10::hip::OptionalHIPGuardMasqueradingAsCUDA device_guard(device_of(kCache));
@@ -195,13 +198,7 @@ void cache_read(const at::Tensor& kCache, const at::Tensor& k, const at::Tensor&
                 const OptTensor& kScales, const OptTensor& vScales) {
     const Tokens t = tokens_of(k, kCache, slots, v, vCache, kScales, vScales);
     check_written(k, "k");
-    check_no_gradient(kCache, "kCache");
-    check_no_gradient(k, "k");
-    if (t.both) {
-        check_written(*v, "v");
-        check_no_gradient(*vCache, "vCache");
-        check_no_gradient(*v, "v");
-    }
+    if (t.both) check_written(*v, "v");
     check_apart({{k, "k"}, {v, "v"}},
                 {{kCache, "kCache"}, {vCache, "vCache"}, {kScales, "kScales"}, {vScales, "vScales"}, {slots, "slots"}});
     const c10::hip::OptionalHIPGuardMasqueradingAsCUDA device_guard(device_of(kCache));
@@ -230,7 +227,10 @@ hfk_attention attention_of(const at::Tensor& q, const at::Tensor& kCache, const 
     check_no_gradient(q, "q");
     check_no_gradient(kCache, "kCache");
     check_no_gradient(vCache, "vCache");
+    check_no_gradient(kScales, "kScales");
+    check_no_gradient(vScales, "vScales");
     check_no_gradient(out, "out");
+    check_no_gradient(lse, "lse");
     TORCH_CHECK(q.size(1) > 0 && q.size(1) <= 0xffffffffLL && q.size(1) % kCache.size(2) == 0, "q has ", q.size(1),
                 " heads, which is no multiple of the cache's ", kCache.size(2));
     TORCH_CHECK(out.scalar_type() == q.scalar_type(), "out must have q's type");

@@ -136,3 +136,29 @@ def test_neighbours_in_one_memory_are_no_overlap():
         back = torch.zeros(2, 3, 2, 64, dtype=BF16, device=DEV)
         ops.cache_read(k, back[0], slots, v, back[1], ks, vs)
         assert bool((back[0] == 1).all()) and bool((back[1] == 2).all())
+
+
+def test_gradients_of_scales_and_of_the_logarithm():
+    """A gradient would have to flow through e4m3 scales and through lse as through the values."""
+    announce("scales and lse that require a gradient")
+    (f, fs), (g, gs) = cache_of(FP8), cache_of(FP8)
+    x, slots = torch.zeros(3, 2, 64, dtype=BF16, device=DEV), torch.arange(3, device=DEV)
+    q, out, lse = torch.zeros(3, 4, 64, dtype=BF16, device=DEV), torch.zeros(3, 4, 64, dtype=BF16, device=DEV), torch.zeros(3, 4, device=DEV)
+    table, starts, lens = torch.zeros(1, 2, dtype=torch.int64, device=DEV), torch.tensor([0, 3], device=DEV), torch.tensor([5], device=DEV)
+
+    def calls(ks, vs, lse):
+        yield "write", lambda: ops.cache_write(x, f, slots, x.clone(), g, ks, vs)
+        yield "read", lambda: ops.cache_read(f, x, slots, g, x.clone(), ks, vs)
+        yield "prompt", lambda: ops.prompt_attention(q, f, g, table, starts, lens, out, 0.1, True, ks, vs, lse)
+        yield "prefix", lambda: ops.prefix_attention(q, f, g, table[0], lens, table.repeat(3, 1), lens.repeat(3), out, 0.1, ks, vs, lse)
+
+    for what, change in (("kScales", dict(ks=fs.clone().requires_grad_())), ("vScales", dict(vs=gs.clone().requires_grad_())),
+                         ("lse", dict(lse=lse.clone().requires_grad_()))):
+        for name, call in calls(**{**dict(ks=fs, vs=gs, lse=lse), **change}):
+            if what == "lse" and name in ("write", "read"):
+                continue
+            with refused(what + " requires a gradient"):
+                call()
+            with torch.no_grad():
+                call()
+    torch.cuda.synchronize()

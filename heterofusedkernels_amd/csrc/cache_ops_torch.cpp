@@ -77,6 +77,7 @@ void check_apart(std::initializer_list<Named> written, std::initializer_list<Nam
 void check_no_gradient(const at::Tensor& t, const char* what) {
     TORCH_CHECK(!(at::GradMode::is_enabled() && t.requires_grad()), what,
                 " requires a gradient, which this op does not compute: detach it or call the op under torch.no_grad()");
+    TORCH_CHECK(!t._fw_grad(0).defined(), what, " carries a tangent, which this op does not pass on: give its primal alone");
 }
 void check_no_gradient(const OptTensor& t, const char* what) {
     if (t.has_value()) check_no_gradient(*t, what);

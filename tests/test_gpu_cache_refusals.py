@@ -162,3 +162,44 @@ def test_gradients_of_scales_and_of_the_logarithm():
             with torch.no_grad():
                 call()
     torch.cuda.synchronize()
+
+
+def test_tangents_of_forward_mode():
+    """The ops have no derivative in either direction: a tangent is refused, not dropped."""
+    import torch.autograd.forward_ad as forward
+
+    announce("tangents")
+    (k, _), (v, _) = cache_of(BF16), cache_of(BF16)
+    (f, fs), (g, gs) = cache_of(FP8), cache_of(FP8)
+    x, slots = torch.zeros(3, 2, 64, dtype=BF16, device=DEV), torch.arange(3, device=DEV)
+    q, out, lse = torch.zeros(3, 4, 64, dtype=BF16, device=DEV), torch.zeros(3, 4, 64, dtype=BF16, device=DEV), torch.zeros(3, 4, device=DEV)
+    table, starts, lens = torch.zeros(1, 2, dtype=torch.int64, device=DEV), torch.tensor([0, 3], device=DEV), torch.tensor([5], device=DEV)
+
+    def attend(q=q, k=k, v=v, out=out, lse=lse, ks=None, vs=None):
+        yield lambda: ops.prompt_attention(q, k, v, table, starts, lens, out, 0.1, True, ks, vs, lse)
+        yield lambda: ops.prefix_attention(q, k, v, table[0], lens, table.repeat(3, 1), lens.repeat(3), out, 0.1, ks, vs, lse)
+
+    def dual(t):
+        return forward.make_dual(t, torch.ones_like(t))
+
+    with forward.dual_level():
+        for name, t in (("q", q), ("k", k), ("v", v), ("out", out), ("lse", lse)):
+            for call in attend(**{name: dual(t)}):
+                with refused({"k": "kCache", "v": "vCache"}.get(name, name) + " carries a tangent"):
+                    call()
+        for name, t in (("ks", fs), ("vs", gs)):
+            for call in attend(**{**dict(k=f, v=g, ks=fs, vs=gs), name: dual(t)}):
+                with refused(name[0] + "Scales carries a tangent"):
+                    call()
+        with refused("k carries a tangent"):
+            ops.cache_write(dual(x), k, slots)
+        with refused("v carries a tangent"):
+            ops.cache_write(x, k, slots, dual(x.clone()), v)
+        with refused("vCache carries a tangent"):
+            ops.cache_read(k, x, slots, dual(v), x.clone())
+        with torch.no_grad():      # which does not switch forward mode off
+            with refused("k carries a tangent"):
+                ops.cache_write(dual(x), k, slots)
+        for call in attend(q=forward.unpack_dual(dual(q)).primal):
+            call()
+    torch.cuda.synchronize()

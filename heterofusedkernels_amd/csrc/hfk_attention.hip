@@ -237,10 +237,13 @@ __device__ uint32_t one_register(uint32_t x) {
 // out = V^T P^T / l with P = exp2(S - m), S = K Q^T * scale * log2 e, over tiles of KEYS keys: bound by the matrix units, with the
 // exponentials, the maximum and the widening of e4m3 on the vector units next to them. 256 rows per workgroup, so that a tile
 // put into LDS once serves eight waves, and two waves per SIMD, so that one has the matrix unit while the other has the vector
-// unit. Measured: a causal prompt of 8192 tokens, 32 heads over 8 of 128 in bf16, 553 to 578 us, 950 to 990 TFLOP/s (matrix units busy 42 %
-// of the cycles; a large matrix product reaches 1580); 250 tokens behind 16000 in e4m3 76 us, 870 TFLOP/s. Without the turns, four
-// waves of 32 rows: 1399 us. Heads of 64: 530 TFLOP/s, as the exponentials weigh twice. Heads of 256 take tiles of 32 keys, since
-// LDS holds no more, and spill about 58 registers: 216 TFLOP/s (4096 tokens, 16 heads over 4).
+// unit. Measured: a causal prompt of 8192 tokens, 32 heads over 8 of 128 in bf16, 563 to 575 us, 960 to 980 TFLOP/s (matrix units busy 41 %
+// of the cycles; a large matrix product reaches 1560 to 1580); 250 tokens behind 16000 in e4m3 81 us in a long series of launches, 90 in its
+// first twenty. Without the turns, four waves of 32 rows: 1399 us. Heads of 64: 610 TFLOP/s, as the exponentials weigh twice. Heads of 256
+// take tiles of 32 keys, since LDS holds no more, and spill about 58 registers: 330 TFLOP/s (211 for 4096 tokens, 16 heads over 4).
+// The weights go into the second product rounded to T: an output's error against 64 bits is 2.1e-3 of the outputs' size in bf16 then, 1.6e-3
+// being the output's own rounding (2.2e-4 and 1.9e-4 in fp16). Their rest as a second operand (see rest8) would take that away and cost the
+// matrix units half as much again: 770 us instead of 574 for the causal prompt, 109 instead of 86.5 for the e4m3 chunk and its join.
 template <typename T, bool FP8, int DP, int KEYS>
 __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(const AttentionArgs a, const WideWalk w) {
     constexpr uint32_t kRows = hfk::kWideRows, kThreads = kWideThreads, kWaves = kThreads / 64;

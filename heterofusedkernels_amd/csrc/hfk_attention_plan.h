@@ -13,7 +13,10 @@
 namespace hfk {
 
 constexpr uint32_t kWideRows = 256;        // query rows of a wide workgroup
-constexpr uint32_t kMinSplitKeys = 256;    // no split of a wide workgroup's keys shorter than this: its fixed cost would show
+// No split of a wide workgroup's keys is shorter than this: its fixed cost would show. (Microseconds with 128 | 256 | 512, 32 heads over 8 of
+// 128: 33 tokens behind 600: 17.6 | 22.4 | 26.6; 250 behind 1000: 30.3 | 29.9 | 37.2; behind 4000: 40.5 all three. 4 heads over 1 of 64, 250
+// behind 2000: 19.3 | 21.5 | 27.3.)
+constexpr uint32_t kMinSplitKeys = 256;
 
 // Cache heads of a narrow workgroup's four waves, and the keys they take at a time.
 inline uint32_t narrow_heads(uint32_t cache_heads) { return cache_heads % 4 == 0 ? 4 : 1; }
@@ -99,6 +102,12 @@ inline PrefixPlan plan_prefix(uint64_t n_rows, uint32_t q_heads, uint32_t cache_
     PrefixPlan p{};
     const uint32_t group = q_heads / cache_heads;
     if (prefix_keys != 0) {
+        // Wide from more rows than one narrow workgroup takes, which would read the prefix again for every tile of rows. Microseconds of
+        // a call under 16384 tokens of 8 heads in bf16, rows per cache head: narrow | wide
+        //   heads of 64:  16: 22.0 | 26.6, 32: 30.1 | 26.8, 64: 38.8 | 27.4,  96: 42.1 | 28.4, 256:  47.7 |  37.3
+        //   heads of 128: 16: 33.5 | 33.0, 32: 44.1 | 33.6, 64: 47.0 | 34.9,  96: 53.4 | 36.7, 256:  68.2 |  46.4
+        //   heads of 256: 16: 54.6 | 94.0, 32: 70.6 | 94.9, 64: 75.8 | 99.4, 128: 87.5 | 123,  256: 125   | 195 (wide spills registers)
+        // The times cross at fewer rows for heads of up to 128, and not at all here for heads of 256.
         p.wide_prefix = n_rows * group > (padded_head_dim(head_dim) == 256 ? 32 : 64);
         if (p.wide_prefix) p.wide = plan_wide(n_rows * group, 1, cache_heads, prefix_keys, 256);
         else p.prefix = plan_narrow(n_rows * group, cache_heads, head_dim, ceil_div(prefix_keys, narrow_unit(cache_heads)));

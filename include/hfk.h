@@ -534,7 +534,8 @@ typedef struct hfk_attention {
  * out (unless it is q) and lse share no memory with each other or with anything that is read.
  * Types: q and out HFK_BF16 or HFK_FP16; the cache of the same type or HFK_FP8_E4M3. Scores, statistics
  * and sums are held in 32 bits. The second product takes the weights in q's type; where a launch waits for
- * memory (few rows per cache head, head_dim up to 128) it takes their rounding error too, as a second operand.
+ * memory (few rows per cache head, head_dim up to 128) it takes their rounding error too, as a second operand. An HFK_FP8_E4M3 cache
+ * is widened to q's type first, as hfk_cache_read does it: with HFK_FP16 values below 2^-14 lose bits and those beyond 65504 become 65504.
  * head_dim: a multiple of 16 up to 256. All pointers and strides multiples of 16 bytes. A block spans less than
  * 4 GiB, a sequence or the prefix has at most 2^30 tokens of table, and no launch has 2^32 threads (n_rows * q_heads / 256 + n_seqs * heads below
  * 2^23 for prompts, n_rows * q_heads below 2^26 for hfk_prefix_attention), else HFK_ERR_TOO_LARGE; the cache itself may be of any size.

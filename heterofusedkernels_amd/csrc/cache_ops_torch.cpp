@@ -66,12 +66,21 @@ void check_apart(std::initializer_list<Named> written, std::initializer_list<Nam
     const auto check = [](const Named& a, const Named& b) {
         if (a.first >= b.end || b.first >= a.end) return;
         const at::MemOverlapStatus s = at::get_overlap_status(*a.tensor, *b.tensor);
-        TORCH_CHECK(s != at::MemOverlapStatus::Partial && s != at::MemOverlapStatus::Full, a.name, " and ", b.name, " must not overlap");
+        TORCH_CHECK(a.first != b.first && s != at::MemOverlapStatus::Partial && s != at::MemOverlapStatus::Full, a.name, " and ", b.name,
+                    " must not overlap");
     };
     for (const Named* w = written.begin(); w != written.end(); ++w) {
         for (const Named* other = w + 1; other != written.end(); ++other) check(*w, *other);
         for (const Named& r : read) check(*w, r);
     }
+}
+
+// Results in place of the queries: every value where its query's was, or nowhere near.
+void check_in_place(const at::Tensor& out, const at::Tensor& q) {
+    bool sound = at::get_overlap_status(out, q) != at::MemOverlapStatus::Partial;
+    if (q.numel() != 0 && out.const_data_ptr() == q.const_data_ptr())
+        for (int64_t i = 0; i < q.dim(); ++i) sound &= q.size(i) == 1 || q.stride(i) == out.stride(i);
+    TORCH_CHECK(sound, "out and q, unless they are one tensor, must not overlap");
 }
 
 void check_no_gradient(const at::Tensor& t, const char* what) {
@@ -222,7 +231,7 @@ hfk_attention attention_of(const at::Tensor& q, const at::Tensor& kCache, const 
     a.q = rows_of(q, kCache, q.size(0), q.size(1), "q");
     a.out = rows_of(out, kCache, q.size(0), q.size(1), "out");
     check_written(out, "out");
-    TORCH_CHECK(at::get_overlap_status(out, q) != at::MemOverlapStatus::Partial, "out and q, unless they are one tensor, must not overlap");
+    check_in_place(out, q);
     check_apart({{lse, "lse"}}, {{q, "q"}});
     check_apart({{out, "out"}, {lse, "lse"}}, {{kCache, "kCache"}, {vCache, "vCache"}, {kScales, "kScales"}, {vScales, "vScales"}});
     check_no_gradient(q, "q");

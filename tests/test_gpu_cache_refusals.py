@@ -203,3 +203,36 @@ def test_tangents_of_forward_mode():
         for call in attend(q=forward.unpack_dual(dual(q)).primal):
             call()
     torch.cuda.synchronize()
+
+
+def test_views_that_begin_at_one_address():
+    """Strided views share memory for certain where they begin at one address, whatever their strides: e4m3 blocks that carry their
+    scales, given for both sides; results that begin where the queries do but lie otherwise."""
+    announce("strided views of one address")
+    x, slots = torch.zeros(3, 2, 64, dtype=BF16, device=DEV), torch.arange(3, device=DEV)
+    raw = torch.zeros(4, pcie_through.fp8_block_bytes(16, 2, 64), dtype=torch.uint8, device=DEV)
+    (k, ks), (again, again_s) = pcie_through.fp8_cache_views(raw, 16, 2, 64), pcie_through.fp8_cache_views(raw, 16, 2, 64)
+    other = torch.ones(4, 16, 2, device=DEV)
+    with refused("kCache and vCache must not overlap"):
+        ops.cache_write(x, k, slots, x.clone(), again, ks, other)
+    (far, _), = [pcie_through.fp8_cache_views(raw.clone(), 16, 2, 64)]
+    with refused("kScales and vScales must not overlap"):
+        ops.cache_write(x, k, slots, x.clone(), far, ks, again_s)
+    wide = torch.zeros(3, 2, 128, dtype=BF16, device=DEV)
+    with refused("k and v must not overlap"):
+        ops.cache_read(k, wide[..., :64], slots, far, wide[..., :64], ks, other)
+
+    buffer = torch.zeros(3, 8, 128, dtype=BF16, device=DEV)
+    q = buffer[:, :4, :64]
+    table, starts, lens = torch.zeros(1, 2, dtype=torch.int64, device=DEV), torch.tensor([0, 3], device=DEV), torch.tensor([5], device=DEV)
+    cache = torch.zeros(4, 16, 2, 64, dtype=BF16, device=DEV)
+    for out in (buffer[:, ::2, :64], buffer.view(6, 4, 128)[:3, :, :64]):
+        with refused("out and q, unless they are one tensor, must not overlap"):
+            ops.prompt_attention(q, cache, cache, table, starts, lens, out, 0.1)
+        with refused("out and q, unless they are one tensor, must not overlap"):
+            ops.prefix_attention(q, cache, cache, table[0], lens, table.repeat(3, 1), lens.repeat(3), out, 0.1)
+    # one view of a wider buffer in place of another of the same strides: results in place of the queries; a stride of one row is no stride
+    ops.prompt_attention(q, cache, cache, table, starts, lens, buffer[:, :4, :64], 0.1)
+    one = buffer[:1, :4, :64]
+    ops.prefix_attention(one, cache, cache, table[0], lens, table, lens, one.as_strided((1, 4, 64), (64, 128, 1)), 0.1)
+    torch.cuda.synchronize()

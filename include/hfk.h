@@ -484,7 +484,7 @@ typedef struct hfk_token_rows {
  *     A power of two makes the division, and the product on the way back, exact: the only error is
  *     the rounding to 4 significant bits.
  * v_plane and v may both be NULL (a cache of one latent tensor per layer); the two sides may differ
- * in heads and head_dim. slots are device-visible; slots of one call must be distinct: of two rows for one slot
+ * in heads and head_dim, not in type. slots are device-visible; slots of one call must be distinct: of two rows for one slot
  * any mixture may be left there, values of one under the scale of the other included.
  * What is written (here planes and scales, in hfk_cache_read the rows) shares no memory with anything else that the call reads or
  * writes: rows are taken in no order. Tokens move within a cache through hfk_cache_read and rows of their own.
